@@ -12,6 +12,7 @@ from .build import LIB
 
 CPG_OK, CPG_EINVAL, CPG_ECUDA, CPG_ETIMEOUT, CPG_ENOMEM, CPG_ENCCL, CPG_ESTATE = 0, -1, -2, -3, -4, -5, -6
 ENC_F32, ENC_Q8, ENC_Q4 = 0, 8, 4
+T_F32, T_F16, T_BF16 = 0, 1, 2
 GROUP_BYTES = {ENC_Q4: 18, ENC_Q8: 34}
 
 # every symbol include/cpg.h declares (tests check the library exports each one)
@@ -34,6 +35,8 @@ EXPORTS = [
     "cpg_qwen3_logits", "cpg_qwen3_stream", "cpg_qwen3_position",
     "cpg_qwen3_batch_create", "cpg_qwen3_batch_destroy", "cpg_qwen3_batch_prefill", "cpg_qwen3_batch_step",
     "cpg_qwen3_batch_generate", "cpg_qwen3_batch_position", "cpg_qwen3_batch_logits",
+    "cpg_kv_create", "cpg_kv_destroy", "cpg_kv_append", "cpg_kv_attend", "cpg_kv_attend_workspace_bytes",
+    "cpg_kv_check",
 ]
 
 
@@ -65,6 +68,20 @@ class Qwen3Desc(ctypes.Structure):
                 ("max_ctx", ctypes.c_int), ("rope_theta", ctypes.c_float), ("rms_eps", ctypes.c_float),
                 ("embed", Tensor), ("lm_head", Tensor), ("final_norm", ctypes.c_void_p),
                 ("attn", ctypes.POINTER(Qwen3Attn)), ("moe", ctypes.POINTER(ctypes.c_void_p))]
+
+
+class KvDesc(ctypes.Structure):
+    _fields_ = [("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("type", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("page_stride", ctypes.c_long), ("pos_stride", ctypes.c_long), ("head_stride", ctypes.c_long),
+                ("rope_dim", ctypes.c_int), ("rope_theta", ctypes.c_float), ("rope_f32", ctypes.c_int)]
+
+
+class KvRows(ctypes.Structure):
+    """cpg_kv_batch."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("rows", ctypes.c_int), ("q_start", ctypes.c_void_p),
+                ("pos0", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("max_new", ctypes.c_int)]
 
 
 class StoreTotals(ctypes.Structure):
@@ -139,6 +156,12 @@ _SIGS = {
     "cpg_qwen3_batch_generate": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
     "cpg_qwen3_batch_position": (_i, [_vp, _i]),
     "cpg_qwen3_batch_logits": (_vp, [_vp, ctypes.POINTER(_i)]),
+    "cpg_kv_create": (_i, [ctypes.POINTER(KvDesc), ctypes.POINTER(_vp)]),
+    "cpg_kv_destroy": (None, [_vp]),
+    "cpg_kv_append": (_i, [_vp, ctypes.POINTER(KvRows), _i, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _f, _vp, _l, _vp]),
+    "cpg_kv_attend_workspace_bytes": (_sz, [_vp, _i]),
+    "cpg_kv_attend": (_i, [_vp, ctypes.POINTER(KvRows), _i, _i, _vp, _l, _vp, _l, _f, _i, _vp, _sz, _vp]),
+    "cpg_kv_check": (_i, [_vp, _vp]),
     "cpg_ctx_x": (_vp, [_vp]),
     "cpg_ctx_topk": (_vp, [_vp]),
     "cpg_ctx_profile": (_i, [_vp, _i]),

@@ -302,6 +302,75 @@ int cpg_qwen3_batch_position(const cpg_qwen3_batch *b, int slot);   /* -1: empty
    prefill's one row. */
 const float *cpg_qwen3_batch_logits(const cpg_qwen3_batch *b, int *rows);
 
+/* ============================================================== paged key/value cache
+ * The cache of many sequences in pools of fixed-size pages, with the two operators of a step:
+ * append (head RMSNorm and position rotation on the way in) and attention of the new rows over
+ * what is cached. The reference keeps one contiguous f32 cache per sequence (qwen3_moe.h:40-70);
+ * per row the arithmetic is qwen3_moe.c:44-49, 110-155 and kernels.c:425-447.
+ *
+ * Element (page, place, head, e) of the key pool lies at k[page·page_stride + place·pos_stride +
+ * head·head_stride + e], of the value pool likewise: any order of the three axes whose positions
+ * do not overlap, strides multiples of 16 bytes. The caller owns the pools and the tables. */
+#define CPG_T_F32  0
+#define CPG_T_F16  1
+#define CPG_T_BF16 2
+typedef struct {
+    int n_kv, head_dim;                  /* cached heads; 64 or 128 */
+    int page_size, n_pages;              /* positions per page, a multiple of 8 */
+    int type;                            /* CPG_T_*: the pools' elements */
+    void *k, *v;                         /* device pools, 16-byte aligned */
+    long page_stride, pos_stride, head_stride;   /* in elements */
+    int rope_dim;                        /* rotated elements of a head: a multiple of 16, 0 = none */
+    float rope_theta;
+    int rope_f32;                        /* 0: angles exact to f32 at any position; 1: the reference's
+                                            f32 angles (kernels.c:425-447), off by up to pos·2^-23 */
+} cpg_kv_desc;
+typedef struct cpg_kv cpg_kv;
+/* The handle belongs to the current device; it keeps a status word there and no other memory. */
+int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out);
+void cpg_kv_destroy(cpg_kv *kv);
+
+/* The rows of a step: sequence i brings rows q_start[i] .. q_start[i+1]-1 (none, one or a chunk of
+ * a prompt), at positions pos0[i], pos0[i]+1, ... The arrays are device memory, read when the
+ * kernels run (a captured call follows them). Rows outside every sequence are left alone: not
+ * appended, their q_out and out rows not written. */
+typedef struct {
+    int n_seqs, rows;                    /* rows of q, k, v and out */
+    const int *q_start;                  /* (n_seqs + 1), ascending */
+    const int *pos0;                     /* (n_seqs) position of the first new row */
+    const int *pages;                    /* (n_seqs, max_pages) page ids, rows table_stride apart */
+    int table_stride, max_pages;
+    int max_new;                         /* most new rows of a sequence; 0: not known. Chooses the
+                                            kernel only: any value gives right results */
+} cpg_kv_batch;
+
+/* Append: keys and values (rows of n_kv heads) into the rows' pages, queries (rows of n_heads; 0:
+ * no queries) to q_out, which may be q. Queries and keys: RMSNorm with gain q_norm / k_norm (f32,
+ * head_dim; NULL: no norm), then the rotation of the first rope_dim elements. Rows are f32 or of
+ * the cache's type; row strides in elements, heads of a row dense, so q, k and v may be parts of
+ * one projection's rows. Arithmetic in f32, each value rounded once. */
+int cpg_kv_append(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads, const void *q, long q_stride,
+                  const void *k, long k_stride, const void *v, long v_stride, const float *q_norm,
+                  const float *k_norm, float eps, void *q_out, long q_out_stride, void *stream);
+
+/* Attention: the row at position p attends to the cached positions j <= p of its sequence, with
+ * window > 0 only to j > p - window; n_heads a multiple of n_kv, consecutive heads sharing a cached
+ * one; weights softmax(scale q·k). Positions behind a sequence's last row are not looked at,
+ * whatever the pages hold there. A position that only some rows of a sequence see takes part in the
+ * others' sums with weight zero, so its value must be finite. out may be q.
+ * f32 rows: products to about 22 bits, f32 sums. 16-bit rows: the weights are rounded to the
+ * cache's type before the sum over values, which accumulates in f32.
+ * ws: device memory of cpg_kv_attend_workspace_bytes, zeroed once before its first use; every call
+ * leaves it ready for the next, of any shape, and calls that overlap need one each. */
+size_t cpg_kv_attend_workspace_bytes(const cpg_kv *kv, int n_heads);
+int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads, const void *q, long q_stride,
+                  void *out, long out_stride, float scale, int window, void *ws, size_t ws_bytes, void *stream);
+/* Synchronise `stream` and report, once, what the calls since the last check met: CPG_EINVAL if a
+ * page id lay outside the pool, or rows or positions outside the batch or its table (such keys and
+ * values were not written, and what the rows that see them hold is not specified; no memory outside
+ * the pools and the rows was touched), CPG_ETIMEOUT if a bounded device wait gave up. */
+int cpg_kv_check(const cpg_kv *kv, void *stream);
+
 /* ============================================================== decode loop (host buffers)
  * A context owns a stream, a workspace and device activation buffers on one device. */
 typedef struct cpg_ctx cpg_ctx;
