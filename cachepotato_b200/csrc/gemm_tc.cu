@@ -548,6 +548,29 @@ static EncodeTiledFn encode_tiled() {
     return fn;
 }
 
+// A tiled map of f32 / f16 / bf16 elements (CPG_T_*), 128-byte swizzle, zeros outside. strides in
+// bytes, of the axes after the first.
+int tensor_map(CUtensorMap *map, int type, int rank, const void *base, const uint64_t *dims, const uint64_t *strides,
+               const uint32_t *box) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) {
+        set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+        return CPG_ECUDA;
+    }
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(map, type == CPG_T_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : type == CPG_T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           rank, const_cast<void *>(base), (const cuuint64_t *)dims, (const cuuint64_t *)strides,
+                           (const cuuint32_t *)box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("tensor map of %d axes failed (%d)", rank, (int)r);
+        return CPG_ECUDA;
+    }
+    return CPG_OK;
+}
+
 int build_row_maps(const uint8_t *const *h_ptrs, int E, int D, int F, int wenc, int rows_gu, int rows_dn,
                    void **d_maps) {
     EncodeTiledFn enc = encode_tiled();

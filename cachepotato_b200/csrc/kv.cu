@@ -10,6 +10,7 @@
 
 struct cpg_kv {
     cpg::KvView v;
+    cpg::KvMaps maps;
     int hd, device, rope_dim, rope_f32;
     float theta;
     double freq[64];                 // theta^(-2j/R) / pi: a position's angle in half turns is p·freq
@@ -173,9 +174,11 @@ static cudaError_t launch_append(int hd, const AppendArgs &a, dim3 grid, dim3 bl
                      : launch_pdl(k_kv_append<TI, TC, 64>, grid, block, 0, s, a);
 }
 
-int kv_attend_launch(const KvView &c, int hd, const KvRows &b, const void *q, size_t q_stride, void *out,
-                     size_t out_stride, int type, int n_heads, float scale, int window, int max_new, void *ws,
+int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &b, const void *q, size_t q_stride,
+                     void *out, size_t out_stride, int type, int n_heads, float scale, int window, int max_new, void *ws,
                      cudaStream_t s);
+int tensor_map(CUtensorMap *map, int type, int rank, const void *base, const uint64_t *dims, const uint64_t *strides,
+               const uint32_t *box);
 size_t kv_attend_ws_bytes(int hd, int type);
 
 static size_t type_bytes(int type) { return type == CPG_T_F32 ? 4 : 2; }
@@ -230,6 +233,19 @@ extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) {
     kv->theta = d->rope_theta;
     for (int j = 0; j < d->rope_dim / 2; ++j)
         kv->freq[j] = pow((double)d->rope_theta, -2.0 * j / d->rope_dim) / 3.14159265358979323846;
+    kv->maps.box = 8;
+    while (kv->maps.box < 64 && d->page_size % (2 * kv->maps.box) == 0) kv->maps.box *= 2;
+    const uint64_t dims[4] = {hd, (uint64_t)d->page_size, (uint64_t)d->n_kv, (uint64_t)d->n_pages};
+    uint64_t ts[3];                                       // an axis of one entry has no stride of its own
+    for (int i = 0; i < 3; ++i) ts[i] = (n[(i + 1) % 3] > 1 ? st[(i + 1) % 3] : (long)hd) * es;
+    const uint32_t box[4] = {(uint32_t)(128 / es), (uint32_t)kv->maps.box, 1, 1};
+    for (int i = 0; i < 2; ++i) {
+        const int rc = tensor_map(&kv->maps.m[i], d->type, 4, i ? d->v : d->k, dims, ts, box);
+        if (rc) {
+            delete kv;
+            return rc;
+        }
+    }
     cudaError_t ce = cudaGetDevice(&kv->device);
     if (ce == cudaSuccess) ce = cudaMalloc(&kv->v.status, sizeof(int));
     if (ce == cudaSuccess) ce = cudaMemset(kv->v.status, 0, sizeof(int));
@@ -346,7 +362,7 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     const size_t need = kv_attend_ws_bytes(kv->hd, kv->v.type);
     CPG_REQUIRE(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, "%s: workspace of %zu bytes at a 256-byte boundary needed, got %zu",
                 fn, need, ws ? ws_bytes : (size_t)0);
-    return kv_attend_launch(kv->v, kv->hd, r, q, q_stride, out, out_stride, type, n_heads, scale, window, b->max_new, ws,
+    return kv_attend_launch(kv->v, kv->maps, kv->hd, r, q, q_stride, out, out_stride, type, n_heads, scale, window, b->max_new, ws,
                             (cudaStream_t)stream);
 }
 

@@ -1,5 +1,6 @@
 // kv.cuh — the paged key/value cache as its kernels see it (kv.cu, kv_attend.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -20,6 +21,13 @@ struct KvRows {
     int n, T;
     const int *q_start, *pos0, *pages;
     int table_stride, max_pages;
+};
+
+// Tensor maps of the two pools: axes (element, place, head, page), a box of 128 bytes by `box`
+// positions, which lie in one page wherever they start at a multiple of box; 128-byte swizzle.
+struct KvMaps {
+    CUtensorMap m[2];
+    int box;
 };
 
 // Status bits a kernel leaves in KvView::status (reported and cleared by cpg_kv_check).

@@ -12,11 +12,16 @@
 //           are tiles of 64 positions. The units of all items, in order, are cut into equal ranges,
 //           one per block: every block has the same number whatever the lengths, and a single long
 //           sequence is spread over the whole GPU. Nothing about lengths is read on the host.
-//   block   Four warps; warp w takes positions 16w..16w+15 of each tile through a ring of its own in
-//           shared memory (16-byte cp.async, NU units of K or V in flight), so no warp waits for
-//           another inside an item and the ring runs on across items. One pass: running maximum and
-//           sum per row in registers, the scores' fragment is the A operand of P·V as it stands.
-//           At an item's end the four warps' (m, l, o) are added in a fixed order.
+//   block   One producer warp, four consumer warps. The producer walks the block's units and keeps a
+//           ring of K and V tiles of 64 positions full by tensor TMA: a box is as many positions as
+//           lie in one page (the largest power of two dividing the page size, at most 64) by 128
+//           bytes, swizzled; a box without a page reads zeros from outside the pool. Consumer warp
+//           w takes positions 16w..16w+15 of every tile; it waits for tiles only, never for another
+//           consumer inside an item, and the ring runs on across items. One pass: running maximum
+//           and sum per row in registers, the scores' fragment is the A operand of P·V as it
+//           stands. At an item's end the four warps' (m, l, o) are added in a fixed order.
+//           Places of a page behind what is cached may hold anything: scores there are replaced,
+//           and so are the values' fragments (a weight of zero does not silence a NaN).
 //   join    A block's part of an item that others share goes to the workspace. Parts are joined in
 //           groups of about the root of their number, each by the block that finishes its group last,
 //           and the groups by the one that finishes last of all: two short steps where one block
@@ -26,7 +31,10 @@
 //           large as the result's own). f32 rows keep about 22 bits: over an f16 cache q (scaled by
 //           a power of two per row) and P are split into two f16 terms; over a bf16 cache into three
 //           bf16 terms; over an f32 cache K and V are split as well (three bf16 terms by truncation,
-//           exact) and the six products of weight 2^-16 and more are kept. All sums are f32.
+//           exact) and the six products of weight 2^-16 and more are kept. The tensor core cuts
+//           off what it adds to an accumulator instead of rounding, so for f32 rows an accumulator
+//           takes few steps, the smallest products first, and is added to the running sum by a
+//           rounded f32 addition (errors 2.9e-6 without that, 4e-7 with it).
 #include <math.h>
 
 #include <algorithm>
@@ -45,7 +53,7 @@ struct AttendArgs {
     size_t q_stride, out_stride;
     int H;
     float scale2;                    // scale · log2(e)
-    int window;
+    int window, box;                 // box: positions of one tensor TMA load
     float *part;                     // 2 slots per block
     int *counters;                   // 2 per block (groups, by slot), then 1 per block (items)
 };
@@ -63,9 +71,34 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes, or zeros where !ok (src is then not read).
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+// d = a·b
+template <bool HALF>
+__device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// 4D tensor TMA load (no multicast) of the box at (x, place, head, page).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int place, int head, int page,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(place), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 // d += a·b, m16n8k16, of f16 (HALF) or bf16 operands.
@@ -108,12 +141,36 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[N]) {
 }
 
 constexpr int KD_WARPS = 4, KD_KEYS = 16, KD_TILE = KD_WARPS * KD_KEYS, KD_ROWS = 16;
-constexpr int KD_RING = 24 * 1024;                       // bytes in a warp's ring
+constexpr int KD_THREADS = (KD_WARPS + 1) * 32;
+constexpr int KD_RING = 96 * 1024;
 constexpr int KD_MAX_GRID = 512;
 template <int HD> constexpr int kd_slot() { return 2 * KD_ROWS + HD / 2 * 32; }   // floats: m, l, o in fragment order
-template <int HD> constexpr int kd_smem() { return KD_WARPS * KD_RING + 2 * kd_slot<HD>() * 4; }
+constexpr int KD_JOIN = 24;                              // parts of one join, at most (root of KD_MAX_GRID)
+// behind the ring: q's terms (f32 rows) and later three quarters of half the warps' sums, both
+// 3 · HD / 16 · 512 bytes; the maxima and sums of what is joined
+template <int HD> constexpr int kd_buf() { return 3 * HD / 16 * 512; }
+template <int HD> constexpr int kd_smem() { return 1008 + KD_RING + kd_buf<HD>() + KD_JOIN * 2 * KD_ROWS * 4; }
 
-// Sequence i's units: KV · row tiles · position tiles (the same for each of its items).
+// a / b of non-negative numbers; nearly always both have 32 bits, which divide in a fifth of the time.
+__device__ __forceinline__ long kd_div(long a, long b) {
+    return ((a | b) >> 32) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// Units 0..U-1 over NB blocks: block b has [start(b), start(b + 1)), the first U % NB one more.
+struct KdCut {
+    long each, more;
+    __device__ __forceinline__ KdCut(long U, long NB) : each(kd_div(U, NB)), more(U - each * NB) {}
+    __device__ __forceinline__ long start(long b) const { return b * each + min(b, more); }
+    __device__ __forceinline__ int owner(long u) const {
+        const long big = more * (each + 1);
+        return (int)(u < big ? kd_div(u, each + 1) : more + kd_div(u - big, each));
+    }
+};
+
+// Sequence i's units: KV · row tiles · (KD_FIXED + position tiles), the same for each of its items.
+// Beginning and ending an item takes a block as long as some three tiles (4 us against 1.4 us for 64
+// bf16 positions), so an item counts for KD_FIXED tiles more than it has: without them the blocks
+// that end one item and begin the next finish last (128K positions, one row: 62 us against 53 us).
+constexpr int KD_FIXED = 3;
 struct KdSeq {
     KvSeq s;
     int rt, nt, lo_t;
@@ -125,13 +182,13 @@ __device__ __forceinline__ KdSeq kd_seq(const AttendArgs &a, int G, int i) {
     q.rt = (int)(((long)q.s.len * G + KD_ROWS - 1) / KD_ROWS);
     q.lo_t = a.window ? max(0, q.s.p0 - a.window + 1) / KD_TILE : 0;
     q.nt = q.s.len ? (q.s.p0 + q.s.len + KD_TILE - 1) / KD_TILE - q.lo_t : 0;
-    q.units = (long)a.c.KV * q.rt * q.nt;
+    q.units = q.nt ? (long)a.c.KV * q.rt * (q.nt + KD_FIXED) : 0;
     return q;
 }
 
 // A place in the order of units: item (seq, row tile, cached head), position tile.
 struct KdCursor {
-    int seq, sub, kt;                // sub = row tile · KV + cached head; kt from 0
+    int seq, sub, kt;                // sub = row tile · KV + cached head; kt from -KD_FIXED
     KdSeq q;
     int r0, nr, lo, hi;              // the row tile: first (row, head) pair, their number, positions seen
     __device__ __forceinline__ void item(const AttendArgs &a, int G) {
@@ -140,9 +197,8 @@ struct KdCursor {
         lo = a.window ? max(0, q.s.p0 + r0 / G - a.window + 1) : 0;
         hi = q.s.p0 + (r0 + nr - 1) / G + 1;
     }
-    __device__ __forceinline__ void next(const AttendArgs &a, int G) {
-        if (++kt < q.nt) return;
-        kt = 0;
+    __device__ __forceinline__ void next_item(const AttendArgs &a, int G) {
+        kt = -KD_FIXED;
         if (++sub < q.rt * a.c.KV) {
             item(a, G);
             return;
@@ -157,154 +213,187 @@ struct KdCursor {
     __device__ __forceinline__ int head(const AttendArgs &a) const { return sub % a.c.KV; }
 };
 
-// Two states of a row pair joined: m, l (rows g and g + 8 of the lane) and NR registers of o.
-template <int NR>
-__device__ __forceinline__ void kd_join(float (&m)[2], float (&l)[2], float (&o)[NR][4], const float (&m2)[2],
-                                        const float (&l2)[2], const float *o2, int stride) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const float mn = fmaxf(m[r], m2[r]), base = mn == -INFINITY ? 0.0f : mn;
-        const float c1 = ex2(m[r] - base), c2 = ex2(m2[r] - base);
-        l[r] = l[r] * c1 + l2[r] * c2;
-        m[r] = mn;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) o[i][2 * r + e] = o[i][2 * r + e] * c1 + o2[(4 * i + 2 * r + e) * stride] * c2;
-    }
-}
-
 template <typename TI, typename TC, int HD>
-__global__ void __launch_bounds__(KD_WARPS * 32, 2) k_kv_attend(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_constant__ AttendArgs a,
+                                                             const __grid_constant__ CUtensorMap tm_k,
+                                                             const __grid_constant__ CUtensorMap tm_v) {
     constexpr bool F32C = std::is_same<TC, float>::value, F32I = std::is_same<TI, float>::value;
     constexpr bool HALF = std::is_same<TC, __half>::value;
     constexpr int NQ = !F32I ? 1 : HALF ? 2 : 3, NK = F32C ? 3 : 1;
-    constexpr int ES = (int)sizeof(TC), ROWB = HD * ES, UNIT = KD_KEYS * ROWB;   // bytes of a key row, of a ring unit
+    constexpr int ES = (int)sizeof(TC), PARTS = HD * ES / 128, UNIT = KD_TILE * HD * ES;  // 128-byte columns; ring unit
     constexpr int NU = KD_RING / UNIT;
-    constexpr int CPR = ROWB / 16, RPI = 32 / CPR;        // 16-byte chunks per row, rows per warp-wide copy
     constexpr int KS = HD / 16, NT = HD / 8;              // k steps of q·k, n tiles of p·v
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long s_scan[KD_WARPS], s_off;
-    __shared__ int s_seq, s_last;
+    constexpr int KU = F32C ? 1 : KS / 2;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t full[NU], empty[NU];
+    __shared__ long s_scan[KD_WARPS + 1], s_off;
+    __shared__ KdSeq s_item;
+    __shared__ int s_seq, s_last, s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.H / a.c.KV;
+    if (tid == 0) {
+        for (int i = 0; i < NU; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], KD_WARPS);
+        }
+        fence_mbar_init();
+        s_abort = 0;
+    }
+    if (tid == KD_WARPS * 32) {
+        prefetch_map(&tm_k);
+        prefetch_map(&tm_v);
+    }
     pdl_wait();
     pdl_launch_dependents();
 
     // ---- this block's range of units, and the item it starts in
+    const int n = a.b.n;
     KdSeq mine{};
-    long sum = 0;
-    for (int i = tid; i < a.b.n; i += KD_WARPS * 32) {
-        mine = kd_seq(a, G, i);
-        sum += mine.units;
-        if (mine.s.bad && blockIdx.x == 0) atomicOr(a.c.status, KV_BAD_POS);
-    }
-    const long own_sum = sum;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_scan[warp] = sum;
-    __syncthreads();
-    long U = 0;
-#pragma unroll
-    for (int w = 0; w < KD_WARPS; ++w) U += s_scan[w];
-    const int NB = (int)min((long)gridDim.x, U);
+    long U = 0, before = 0, u0 = 0, u1 = 0;
+    int NB = 0;
     const int blk = blockIdx.x;
-    if (blk >= NB) return;
-    const long u0 = U * blk / NB, u1 = U * (blk + 1) / NB;
-    long before = 0;
-    for (int c0 = 0;; c0 += KD_WARPS * 32) {              // a chunk of sequences at a time; U > u0, so it ends
-        long x = own_sum;
-        if (a.b.n > KD_WARPS * 32) x = c0 + tid < a.b.n ? kd_seq(a, G, c0 + tid).units : 0;
-        long inc = x;
+    KdCut cut(0, 1);
+    auto range = [&](long total) {                        // false: nothing for this block
+        U = total;
+        NB = (int)min((long)gridDim.x, U);
+        if (blk >= NB) return false;
+        cut = KdCut(U, NB);
+        u0 = cut.start(blk);
+        u1 = cut.start(blk + 1);
+        return true;
+    };
+    if (n > KD_THREADS) {                                 // more sequences than threads: their sum first
+        long sum = 0;
+        for (int i = tid; i < n; i += KD_THREADS) sum += kd_seq(a, G, i).units;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_scan[warp] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w <= KD_WARPS; ++w) sum += s_scan[w];
+        if (!range(sum)) return;
+        __syncthreads();
+    }
+    for (int c0 = 0; c0 < n; c0 += KD_THREADS) {          // THREADS sequences at a time
+        long inc = 0;
+        if (c0 + tid < n) {
+            mine = kd_seq(a, G, c0 + tid);
+            inc = mine.units;
+            if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
+        }
+        const long x = inc;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long y = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += y;
         }
-        __syncthreads();
         if (lane == 31) s_scan[warp] = inc;
         __syncthreads();
         long base = before, all = 0;
 #pragma unroll
-        for (int w = 0; w < KD_WARPS; ++w) {
+        for (int w = 0; w <= KD_WARPS; ++w) {
             if (w < warp) base += s_scan[w];
             all += s_scan[w];
         }
-        if (u0 >= base + inc - x && u0 < base + inc) {
+        if (n <= KD_THREADS && !range(all)) return;
+        if (c0 + tid < n && u0 >= base + inc - x && u0 < base + inc) {
             s_seq = c0 + tid;
             s_off = u0 - (base + inc - x);
+            s_item = mine;
         }
         before += all;
+        __syncthreads();
         if (u0 < before) break;
     }
-    __syncthreads();
+    if (u0 >= u1) return;                                 // no sequences at all
     KdCursor cur;
     cur.seq = s_seq;
-    cur.q = kd_seq(a, G, cur.seq);
-    cur.sub = (int)(s_off / cur.q.nt);
-    cur.kt = (int)(s_off - (long)cur.sub * cur.q.nt);
+    cur.q = s_item;
+    cur.sub = (int)kd_div(s_off, cur.q.nt + KD_FIXED);
+    cur.kt = (int)(s_off - (long)cur.sub * (cur.q.nt + KD_FIXED)) - KD_FIXED;
     cur.item(a, G);
-    KdCursor ld = cur;
-    long ul = u0;                                         // unit pair (K, V) the loader is at
-    bool ld_v = false;
+    volatile int *const abort_flag = &s_abort;
 
-    const uint32_t ring = smem_u32(smem) + warp * KD_RING;
-    float *const s_o = reinterpret_cast<float *>(smem + KD_WARPS * KD_RING);
-    size_t off[2] = {0, 0};
-    bool ok[2] = {false, false};
-    int vis_lo = 0, vis_hi = 0, slot_ld = 0;
-    // one ring unit: this warp's 16 keys of the loader's tile, K first, then V
-    auto load_unit = [&]() {
-        if (ul < u1) {
-            const int j0 = (ld.q.lo_t + ld.kt) * KD_TILE + warp * KD_KEYS;
-            if (!ld_v) {
-                vis_lo = ld.lo - j0;
-                vis_hi = ld.hi - j0;
+    if (warp == KD_WARPS) {
+        // ---- producer: lane b loads box b of every unit (box = position group · PARTS + column)
+        const int groups = KD_TILE / a.box;
+        const uint32_t ring = smem_u32(smem);
+        int slot = 0, turn = 0;
+        for (long u = u0; u < u1; ++u) {
+            if (cur.kt < 0) {                             // nothing to load
+                ++cur.kt;
+                continue;
+            }
+            const int j0 = (cur.q.lo_t + cur.kt) * KD_TILE;
+            const int boxes = groups * PARTS;
+            int page[2], place[2];                        // boxes lane, lane + 32 (at most 8 groups of 4)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {             // pages hold multiples of 8 positions
-                    ok[x] = 8 * x < vis_hi && 8 * x + 8 > vis_lo;
-                    if (ok[x]) {
-                        const int pg = (j0 + 8 * x) / a.c.P;
-                        const int page = a.b.pages[(size_t)ld.seq * a.b.table_stride + pg];
-                        ok[x] = page >= 0 && page < a.c.n_pages;
-                        if (!ok[x] && lane == 0) atomicOr(a.c.status, KV_BAD_PAGE);
-                        off[x] = ok[x] ? (size_t)page * a.c.sp + (size_t)(j0 + 8 * x - pg * a.c.P) * a.c.st +
-                                             (size_t)ld.head(a) * a.c.sh : 0;
-                    }
+            for (int x = 0; x < 2; ++x) {
+                const int bx = lane + 32 * x, j = j0 + bx / PARTS * a.box;
+                page[x] = a.c.n_pages;                    // outside the pool: zeros
+                place[x] = 0;
+                if (bx < boxes && j < cur.hi && j + a.box > cur.lo) {
+                    const int pg = j / a.c.P;
+                    const int id = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
+                    if (id >= 0 && id < a.c.n_pages) page[x] = id;
+                    else atomicOr(a.c.status, KV_BAD_PAGE);
+                    place[x] = j - pg * a.c.P;
                 }
             }
-            if (vis_hi > 0 && vis_lo < KD_KEYS) {
-                const TC *base = (const TC *)(ld_v ? a.c.v : a.c.k);
-                const int c = lane % CPR;
 #pragma unroll
-                for (int i = 0; i < KD_KEYS / RPI; ++i) {
-                    const int r = i * RPI + lane / CPR;
-                    const int sw = !F32C ? (r & 7) : ld_v ? ((r >> 1) & 3) * 2 : (r & 1) * 4;
-                    const bool in = ok[r >> 3] && r < vis_hi && r >= vis_lo;
-                    const TC *src = in ? base + off[r >> 3] + (size_t)(r & 7) * a.c.st + c * (16 / ES) : base;
-                    cp_async16_or_zero(ring + slot_ld * UNIT + r * ROWB + ((c ^ sw) << 4), src, in);
+            for (int half = 0; half < 2; ++half) {        // K, then V
+                if (turn && !mbar_wait(&empty[slot], (uint32_t)(turn - 1) & 1u)) {
+                    *abort_flag = 1;
+                    atomicOr(a.c.status, KV_TIMEOUT);
+                }
+                if (*abort_flag) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int bx = lane + 32 * x, part = bx % PARTS;
+                    if (bx < boxes)
+                        tma_load_4d(ring + slot * UNIT + part * (KD_TILE * 128) + bx / PARTS * a.box * 128, half ? &tm_v : &tm_k,
+                                    part * (128 / ES), place[x], cur.head(a), page[x], &full[slot]);
+                }
+                if (++slot == NU) {
+                    slot = 0;
+                    ++turn;
                 }
             }
-            if (ld_v) {
-                if (++ul < u1) ld.next(a, G);
-            }
-            ld_v = !ld_v;
+            if (*abort_flag) break;
+            if (++cur.kt == cur.q.nt && u + 1 < u1) cur.next_item(a, G);
         }
-        cp_async_commit();
-        slot_ld = slot_ld + 1 == NU ? 0 : slot_ld + 1;
-    };
-#pragma unroll 1
-    for (int i = 0; i < NU - 1; ++i) load_unit();
+        if (*abort_flag) {                                // copies in flight land before the block may end
+            for (int i = 0; i < NU; ++i) {
+                const int n = turn + (i < slot);          // fills of slot i
+                if (n) mbar_wait(&full[i], (uint32_t)(n - 1) & 1u);
+            }
+        }
+        return;
+    }
 
-    uint32_t qa[NQ][KS][4];
+    // ---- consumers
+    const uint32_t ring = smem_u32(smem);
+    float *const s_o = reinterpret_cast<float *>(smem + KD_RING);
+    uint4 *const s_q = reinterpret_cast<uint4 *>(s_o);    // f32 rows: q's terms in fragment order
+    uint32_t qa[NQ == 1 ? KS : 1][4];
     float o[NT][4], m[2], l[2], sc[2];
     int p_row[2];
-    bool fresh = true;
     int slot = 0;
-    for (long u = u0; u < u1; ++u) {
-        if (fresh) {                                      // a new item: its rows of q, empty sums
-            fresh = false;
+    uint32_t phase = 0;
+    for (long u = u0; u < u1;) {
+        if (cur.kt < 0) {
+            u -= cur.kt;
+            cur.kt = 0;
+            if (u >= u1) break;                           // its first tile is the next block's
+        }
+        {                                                 // an item: its rows of q, empty sums
             const int kh = cur.head(a);
+            float f[2][F32I ? KS : 1][4];
+            float up[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int rr = cur.r0 + g + 8 * r;
@@ -313,316 +402,434 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 2) k_kv_attend(const __grid_con
                 p_row[r] = live ? cur.q.s.p0 + tok : cur.hi - 1;
                 const TI *src = (const TI *)a.q + (size_t)(cur.q.s.r0 + tok) * a.q_stride + (size_t)(kh * G + rr - tok * G) * HD;
                 sc[r] = a.scale2;
+                up[r] = 1.0f;
                 if constexpr (!F32I) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                         for (int x = 0; x < 2; ++x)
-                            qa[0][ks][r + 2 * x] = live ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 8 * x + 2 * t) : 0u;
+                            qa[ks][r + 2 * x] = live ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 8 * x + 2 * t) : 0u;
                 } else {
-                    float f[KS][4];
                     float mx = 0.0f;
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
-                        // f32 cache: K is read four elements a lane, so step ks of lane t is elements
-                        // 4t..4t+3 of the 16; otherwise 2t, 2t+1 and 8 further
+                        // f32 cache: K is read four elements a lane; step 2i + b of lane t is elements
+                        // 32i + 8t + 4b.. (conflict-free); otherwise 16ks + 2t, + 1 and 8 further
                         if constexpr (F32C) {
-                            const float4 v = live ? *reinterpret_cast<const float4 *>(src + 16 * ks + 4 * t) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            f[ks][0] = v.x; f[ks][1] = v.y; f[ks][2] = v.z; f[ks][3] = v.w;
+                            const float4 v = live ? *reinterpret_cast<const float4 *>(src + 32 * (ks / 2) + 8 * t + 4 * (ks & 1))
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                            f[r][ks][0] = v.x; f[r][ks][1] = v.y; f[r][ks][2] = v.z; f[r][ks][3] = v.w;
                         } else {
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
                                 const float2 v = live ? *reinterpret_cast<const float2 *>(src + 16 * ks + 8 * x + 2 * t) : make_float2(0.f, 0.f);
-                                f[ks][2 * x] = v.x;
-                                f[ks][2 * x + 1] = v.y;
+                                f[r][ks][2 * x] = v.x;
+                                f[r][ks][2 * x + 1] = v.y;
                             }
                         }
-                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(f[ks][0]), fabsf(f[ks][1])), fmaxf(fabsf(f[ks][2]), fabsf(f[ks][3]))));
+                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(f[r][ks][0]), fabsf(f[r][ks][1])), fmaxf(fabsf(f[r][ks][2]), fabsf(f[r][ks][3]))));
                     }
-                    float s = 1.0f;
                     if constexpr (HALF) {                 // the row into f16's range by a power of two
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                         const int eb = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
-                        s = __uint_as_float((uint32_t)(254 - eb) << 23);
+                        up[r] = __uint_as_float((uint32_t)(254 - eb) << 23);
                         sc[r] = a.scale2 * __uint_as_float((uint32_t)eb << 23);
                     }
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            uint32_t tm[NQ];
-                            split_pair<HALF, NQ>(f[ks][2 * x] * s, f[ks][2 * x + 1] * s, tm);
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n) qa[n][ks][r + 2 * x] = tm[n];
-                        }
                 }
                 m[r] = -INFINITY;
                 l[r] = 0.0f;
             }
+            if constexpr (F32I) {                         // warp w writes the steps w, w + 4, ... of all terms
+#pragma unroll
+                for (int k4 = 0; k4 < KS / 4; ++k4) {
+                    uint32_t w[NQ][4];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t tm[NQ];
+                            float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                if (warp == y) {
+                                    lo = f[r][4 * k4 + y][2 * x];
+                                    hi = f[r][4 * k4 + y][2 * x + 1];
+                                }
+                            split_pair<HALF, NQ>(lo * up[r], hi * up[r], tm);
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n) w[n][r + 2 * x] = tm[n];
+                        }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        s_q[(n * KS + 4 * k4 + warp) * 32 + lane] = make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]);
+                }
+                named_bar_sync(1, KD_WARPS * 32);
+            }
 #pragma unroll
             for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         }
-        const int j0 = (cur.q.lo_t + cur.kt) * KD_TILE + warp * KD_KEYS;
-        const bool active = j0 < cur.hi && j0 + KD_KEYS > cur.lo;
-        float s[2][4];
+        const int n_here = (int)min((long)(cur.q.nt - cur.kt), u1 - u);          // this block's tiles of it
+        int j0 = (cur.q.lo_t + cur.kt) * KD_TILE + warp * KD_KEYS;
+#pragma unroll 1
+        for (int left = n_here; left > 0; --left, j0 += KD_TILE) {
+            const bool active = j0 < cur.hi && j0 + KD_KEYS > cur.lo;
+            float s[2][4], c[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {            // K, then V
-            load_unit();
-            cp_async_wait_group<NU - 1>();
-            __syncwarp();
-            const uint32_t at = ring + slot * UNIT;
-            if (active && half == 0) {
+            for (int half = 0; half < 2; ++half) {            // K, then V
+                if (!*abort_flag && !mbar_wait(&full[slot], phase)) {
+                    *abort_flag = 1;                          // from here on nothing waits; results are void
+                    atomicOr(a.c.status, KV_TIMEOUT);
+                }
+                const uint32_t at = ring + slot * UNIT + warp * (KD_KEYS * 128);
+                if (active && half == 0) {
+                    float big[2][2][4] = {}, low[2][4] = {};  // f32 rows: large products in two chains, small ones
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                    for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                    // f32 cache: not unrolled, for a short step's time is in fetching its code
+#pragma unroll KU
+                    for (int k2 = 0; k2 < KS / 2; ++k2) {     // 32 elements
+                        uint32_t q2[NQ][2][4];
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                if constexpr (NQ == 1) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) q2[q][b][e] = qa[2 * k2 + b][e];
+                                } else {
+                                    const uint4 v = s_q[(q * KS + 2 * k2 + b) * 32 + lane];
+                                    q2[q][b][0] = v.x; q2[q][b][1] = v.y; q2[q][b][2] = v.z; q2[q][b][3] = v.w;
+                                }
+                            }
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            if constexpr (!F32C) {
+                                const int r = 8 * n + (lane & 7), ch = 4 * k2 + (lane >> 3);
+                                uint32_t b[4];
+                                ldsm4(b, at + ch / 8 * (KD_TILE * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                                if constexpr (NQ == 1) {
+                                    mma_acc<HALF>(s[n], q2[0][0], b[0], b[1]);
+                                    mma_acc<HALF>(s[n], q2[0][1], b[2], b[3]);
+                                } else {
+                                    mma_acc<HALF>(big[n][0], q2[0][0], b[0], b[1]);
+                                    mma_acc<HALF>(big[n][1], q2[0][1], b[2], b[3]);
+#pragma unroll
+                                    for (int q = NQ - 1; q >= 1; --q) {
+                                        mma_acc<HALF>(low[n], q2[q][0], b[0], b[1]);
+                                        mma_acc<HALF>(low[n], q2[q][1], b[2], b[3]);
+                                    }
+                                }
+                            } else {
+                                const int r = 8 * n + g;
+#pragma unroll
+                                for (int b = 0; b < 2; ++b) {
+                                    const float4 v = lds4(at + k2 * (KD_TILE * 128) + r * 128 + (((2 * t + b) ^ (r & 7)) << 4));
+                                    uint32_t b0[NK], b1[NK];
+                                    split_pair<HALF, NK>(v.x, v.y, b0);
+                                    split_pair<HALF, NK>(v.z, v.w, b1);
+                                    mma_acc<HALF>(big[n][b], q2[0][b], b0[0], b1[0]);
+#pragma unroll
+                                    for (int d = NK - 1; d >= 1; --d)      // terms of weight 2^-8d
+#pragma unroll
+                                        for (int k = 0; k <= d; ++k) mma_acc<HALF>(low[n], q2[d - k][b], b0[k], b1[k]);
+                                }
+                            }
+                        }
+                    }
+                    if constexpr (NQ > 1) {
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[n][e] = (big[n][0][e] + big[n][1][e]) + low[n][e];
+                    }
+                    const int span = (cur.nr - 1) / G + 1;    // positions between the tile's rows, at most
+                    if (j0 + KD_KEYS > cur.hi - span || (a.window && j0 < cur.lo + span)) {
+                        // some row of the tile does not see all 16
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int j = j0 + 8 * n + 2 * t + (e & 1), p = p_row[e >> 1];
+                                if (j > p || (a.window && j <= p - a.window)) s[n][e] = -INFINITY;
+                            }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        const float mn = fmaxf(m[r], mx * sc[r]), base = mn == -INFINITY ? 0.0f : mn;
+                        c[r] = ex2(m[r] - base);
+                        m[r] = mn;
+                        float add = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 2 * r; e < 2 * r + 2; ++e) {
+                                s[n][e] = ex2(fmaf(s[n][e], sc[r], -base));
+                                add += s[n][e];
+                            }
+                        l[r] = fmaf(l[r], c[r], add);
+                    }
+                    if constexpr (NQ == 1) {
+                        if (__any_sync(0xffffffffu, c[0] != 1.0f || c[1] != 1.0f)) {
+#pragma unroll
+                            for (int i = 0; i < NT; ++i) {
+                                o[i][0] *= c[0]; o[i][1] *= c[0];
+                                o[i][2] *= c[1]; o[i][3] *= c[1];
+                            }
+                        }
+                    }
+                } else if (active) {
+                    uint32_t pa[NQ][4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            uint32_t tm[NQ];
+                            split_pair<HALF, NQ>(s[n][2 * r], s[n][2 * r + 1], tm);
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q) pa[q][r + 2 * n] = tm[q];
+                        }
+                    // keys 2t, 2t+1, 2t+8, 2t+9 of this lane's fragments that nobody sees
+                    bool hide[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int j = j0 + 2 * t + (y & 1) + 8 * (y >> 1);
+                        hide[y] = j >= cur.hi || j < cur.lo;
+                    }
+                    const bool any = j0 + KD_KEYS > cur.hi || j0 < cur.lo;
+                    // f32 rows: o = o·c + sum, rounded
+                    auto add_to = [&](float (&to)[4], const float (&sum)[4]) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) to[e] = fmaf(to[e], c[e >> 1], sum[e]);
+                    };
                     if constexpr (!F32C) {
-                        const int r = 8 * n + (lane & 7);
+                        const uint32_t k0 = (hide[0] ? 0u : 0xffffu) | (hide[1] ? 0u : 0xffff0000u);
+                        const uint32_t k1 = (hide[2] ? 0u : 0xffffu) | (hide[3] ? 0u : 0xffff0000u);
+                        const int r = lane & 15;
 #pragma unroll
-                        for (int k2 = 0; k2 < KS / 2; ++k2) {
+                        for (int n2 = 0; n2 < NT / 2; ++n2) {
+                            const int ch = 2 * n2 + (lane >> 4);
                             uint32_t b[4];
-                            ldsm4(b, at + r * ROWB + (((4 * k2 + (lane >> 3)) ^ (r & 7)) << 4));
+                            ldsm4t(b, at + ch / 8 * (KD_TILE * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                            if (any) {
+                                b[0] &= k0; b[1] &= k1;
+                                b[2] &= k0; b[3] &= k1;
+                            }
+                            if constexpr (NQ == 1) {
+                                mma_acc<HALF>(o[2 * n2], pa[0], b[0], b[1]);
+                                mma_acc<HALF>(o[2 * n2 + 1], pa[0], b[2], b[3]);
+                            } else {
 #pragma unroll
-                            for (int q = NQ - 1; q >= 0; --q) {
-                                mma_acc<HALF>(s[n], qa[q][2 * k2], b[0], b[1]);
-                                mma_acc<HALF>(s[n], qa[q][2 * k2 + 1], b[2], b[3]);
+                                for (int x = 0; x < 2; ++x) {
+                                    float sum[4];
+                                    mma_new<HALF>(sum, pa[NQ - 1], b[2 * x], b[2 * x + 1]);
+#pragma unroll
+                                    for (int q = NQ - 2; q >= 0; --q) mma_acc<HALF>(sum, pa[q], b[2 * x], b[2 * x + 1]);
+                                    add_to(o[2 * n2 + x], sum);
+                                }
                             }
                         }
                     } else {
-                        const int r = 8 * n + g;
+                        // lane (g, t) reads columns 32cb + 4g.. of its four keys: n tile 4cb + x is the
+                        // columns 32cb + 4n + x
 #pragma unroll
-                        for (int ks = 0; ks < KS; ++ks) {
-                            float4 v;
-                            asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                                         : "r"(at + r * ROWB + (((4 * ks + t) ^ ((r & 1) * 4)) << 4)));
-                            uint32_t b0[NK], b1[NK];
-                            split_pair<HALF, NK>(v.x, v.y, b0);
-                            split_pair<HALF, NK>(v.z, v.w, b1);
+                        for (int cb = 0; cb < HD / 32; ++cb) {
+                            float v[4][4];
 #pragma unroll
-                            for (int d = NK - 1; d >= 0; --d)          // terms of weight 2^-8d
+                            for (int y = 0; y < 4; ++y) {
+                                const int r = 2 * t + (y & 1) + 8 * (y >> 1);
+                                const float4 w = lds4(at + cb * (KD_TILE * 128) + r * 128 + ((g ^ (r & 7)) << 4));
+                                v[y][0] = w.x; v[y][1] = w.y; v[y][2] = w.z; v[y][3] = w.w;
+                                if (any && hide[y]) v[y][0] = v[y][1] = v[y][2] = v[y][3] = 0.0f;
+                            }
 #pragma unroll
-                                for (int k = 0; k <= d; ++k) mma_acc<HALF>(s[n], qa[d - k][ks], b0[k], b1[k]);
+                            for (int x = 0; x < 4; ++x) {
+                                uint32_t b0[NK], b1[NK];
+                                split_pair<HALF, NK>(v[0][x], v[1][x], b0);
+                                split_pair<HALF, NK>(v[2][x], v[3][x], b1);
+                                float sum[4];
+                                mma_new<HALF>(sum, pa[NK - 1], b0[0], b1[0]);          // smallest products first
+#pragma unroll
+                                for (int d = NK - 1; d >= 0; --d)
+#pragma unroll
+                                    for (int k = d == NK - 1; k <= d; ++k) mma_acc<HALF>(sum, pa[d - k], b0[k], b1[k]);
+                                add_to(o[4 * cb + x], sum);
+                            }
                         }
                     }
                 }
-                const int span = (cur.nr - 1) / G + 1;      // positions between the tile's rows, at most
-                const bool cut = j0 + KD_KEYS > cur.hi - span || (a.window && j0 < cur.lo + span);
-                if (cut) {                                // some row of the tile does not see all 16
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = j0 + 8 * n + 2 * t + (e & 1), p = p_row[e >> 1];
-                            if (j > p || (a.window && j <= p - a.window)) s[n][e] = -INFINITY;
-                        }
-                }
-                float c[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    const float mn = fmaxf(m[r], mx * sc[r]), base = mn == -INFINITY ? 0.0f : mn;
-                    c[r] = ex2(m[r] - base);
-                    m[r] = mn;
-                    float add = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 2 * r; e < 2 * r + 2; ++e) {
-                            s[n][e] = ex2(fmaf(s[n][e], sc[r], -base));
-                            add += s[n][e];
-                        }
-                    l[r] = fmaf(l[r], c[r], add);
-                }
-                if (__any_sync(0xffffffffu, c[0] != 1.0f || c[1] != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        o[i][0] *= c[0]; o[i][1] *= c[0];
-                        o[i][2] *= c[1]; o[i][3] *= c[1];
-                    }
-                }
-            } else if (active) {
-                uint32_t pa[NQ][4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        uint32_t tm[NQ];
-                        split_pair<HALF, NQ>(s[n][2 * r], s[n][2 * r + 1], tm);
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) pa[q][r + 2 * n] = tm[q];
-                    }
-                if constexpr (!F32C) {
-                    const int r = lane & 15;
-#pragma unroll
-                    for (int n2 = 0; n2 < NT / 2; ++n2) {
-                        uint32_t b[4];
-                        ldsm4t(b, at + r * ROWB + (((2 * n2 + (lane >> 4)) ^ (r & 7)) << 4));
-#pragma unroll
-                        for (int q = NQ - 1; q >= 0; --q) {
-                            mma_acc<HALF>(o[2 * n2], pa[q], b[0], b[1]);
-                            mma_acc<HALF>(o[2 * n2 + 1], pa[q], b[2], b[3]);
-                        }
-                    }
-                } else {
-                    // lane (g, t) reads columns 32cb + 4g.. of keys 2t, 2t+1, 2t+8, 2t+9: n tile 4cb + x
-                    // is the columns 32cb + 4n + x
-#pragma unroll
-                    for (int cb = 0; cb < HD / 32; ++cb) {
-                        float v[4][4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const int r = 2 * t + (y & 1) + 8 * (y >> 1);
-                            asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                                         : "=f"(v[y][0]), "=f"(v[y][1]), "=f"(v[y][2]), "=f"(v[y][3])
-                                         : "r"(at + r * ROWB + (((8 * cb + g) ^ (((r >> 1) & 3) * 2)) << 4)));
-                        }
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            uint32_t b0[NK], b1[NK];
-                            split_pair<HALF, NK>(v[0][x], v[1][x], b0);
-                            split_pair<HALF, NK>(v[2][x], v[3][x], b1);
-#pragma unroll
-                            for (int d = NK - 1; d >= 0; --d)
-#pragma unroll
-                                for (int k = 0; k <= d; ++k) mma_acc<HALF>(o[4 * cb + x], pa[d - k], b0[k], b1[k]);
-                        }
-                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[slot]);
+                if (++slot == NU) {
+                    slot = 0;
+                    phase ^= 1;
                 }
             }
-            __syncwarp();
-            slot = slot + 1 == NU ? 0 : slot + 1;
-        }
-        const bool item_ends = cur.kt + 1 == cur.q.nt;
-        if (!item_ends && u + 1 < u1) {
-            cur.next(a, G);
-            continue;
         }
 
-        // ---- the item, or this block's part of it, is done: join the four warps
+        // ---- the item, or this block's part of it, is done. The warps' sums are brought to the
+        // common maximum and added so that each warp ends with a quarter of the columns: half the
+        // n tiles of every quarter at a time, through shared memory
+        constexpr int NQT = NT / 4;                       // n tiles of a quarter
+        float *const s_m = s_o + kd_buf<HD>() / 4, *const s_l = s_m + KD_JOIN * KD_ROWS;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
-        auto put = [&](float *to) {                       // m, l and o in fragment order
             if (t == 0) {
+                s_m[warp * KD_ROWS + g + 8 * r] = m[r];
+                s_l[warp * KD_ROWS + g + 8 * r] = l[r];
+            }
+        }
+        // the largest maximum of n states in s_m, and the sum of s_l for it
+        auto common = [&](int n_states) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    to[g + 8 * r] = m[r];
-                    to[KD_ROWS + g + 8 * r] = l[r];
+            for (int r = 0; r < 2; ++r) {
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
+                for (int k = 0; k < n_states; ++k) m[r] = fmaxf(m[r], s_m[k * KD_ROWS + g + 8 * r]);
+                const float base = m[r] == -INFINITY ? 0.0f : m[r];
+                for (int k = 0; k < n_states; ++k)
+                    l[r] = fmaf(ex2(s_m[k * KD_ROWS + g + 8 * r] - base), s_l[k * KD_ROWS + g + 8 * r], l[r]);
+            }
+        };
+        {
+            const float own[2] = {m[0], m[1]};
+            named_bar_sync(1, KD_WARPS * 32);             // and q's terms are no longer read
+            common(KD_WARPS);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float f = m[r] == -INFINITY ? 0.0f : ex2(own[r] - m[r]);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    o[i][2 * r] *= f;
+                    o[i][2 * r + 1] *= f;
                 }
             }
+        }
+        float oq[NQT][4];
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) to[2 * KD_ROWS + (4 * i + e) * 32 + lane] = o[i][e];
-        };
-        auto add = [&](const float *from) {
-            const float m2[2] = {from[g], from[g + 8]}, l2[2] = {from[KD_ROWS + g], from[KD_ROWS + g + 8]};
-            kd_join<NT>(m, l, o, m2, l2, from + 2 * KD_ROWS + lane, 32);
-        };
-        if (warp >= 2) put(s_o + (warp - 2) * kd_slot<HD>());
-        __syncthreads();
-        if (warp < 2) add(s_o + warp * kd_slot<HD>());
-        __syncthreads();
-        if (warp == 1) put(s_o);
-        __syncthreads();
-        if (warp == 0) add(s_o);
+            for (int w = 0; w < KD_WARPS; ++w)
+                if (w != warp) {
+#pragma unroll
+                    for (int i = 0; i < NQT / 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s_o[((w * 3 + (warp < w ? warp : warp - 1)) * (NQT / 2 * 4) + 4 * i + e) * 32 + lane] = o[w * NQT + h * (NQT / 2) + i][e];
+                }
+            named_bar_sync(1, KD_WARPS * 32);
+#pragma unroll
+            for (int i = 0; i < NQT / 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < KD_WARPS; ++w) {
+                        float v = 0.0f;
+                        if (w != warp) v = s_o[((warp * 3 + (w < warp ? w : w - 1)) * (NQT / 2 * 4) + 4 * i + e) * 32 + lane];
+                        else {
+#pragma unroll
+                            for (int x = 0; x < KD_WARPS; ++x)
+                                if (x == warp) v = o[x * NQT + h * (NQT / 2) + i][e];
+                        }
+                        sum += v;
+                    }
+                    oq[h * (NQT / 2) + i][e] = sum;
+                }
+            named_bar_sync(1, KD_WARPS * 32);
+        }
 
-        // ---- who else has a part of it: unit range [ua, ue) of the item, owners b0..b1
+        // ---- who else has a part of it: the item's tiles are units [ua, ue), blocks b0..b1
         const long ua = u - cur.kt, ue = ua + cur.q.nt;
-        const int b0 = (int)(((ua + 1) * NB - 1) / U), b1 = (int)((ue * NB - 1) / U);
+        u += n_here;
+        const int b0 = cut.owner(ua), b1 = cut.owner(ue - 1);
         bool write = b0 == b1;
         if (!write) {
             const int np = b1 - b0 + 1, p = blk - b0;
-            int gs = 1;
-            while (gs * gs < np) ++gs;
-            if (np <= 8) gs = np;
+            int gs = np;
+            if (np > 16)
+                for (gs = 4; gs * gs < np;) ++gs;
             const int ng = (np + gs - 1) / gs, gi = p / gs, n_in = min(gs, np - gi * gs);
-            auto slot_of = [&](int part) { return (size_t)(part == 0 ? 2 * b0 + 1 : 2 * (b0 + part)); };
-            if (warp == 0) put(a.part + slot_of(p) * kd_slot<HD>());
-            // parts first, first + step, ... (n of them) joined by this block if it is the last of `want`
-            auto join = [&](int *counter, int want, int first, int step, int n) -> bool {
-                if (warp == 0) {
-                    __threadfence();
-                    __syncwarp();
-                    int last = 0;
-                    if (lane == 0) {
-                        last = atomicAdd(counter, 1) == want - 1;
-                        if (last) *counter = 0;           // ready for the next call
-                        __threadfence();
-                    }
-                    if (lane == 0) s_last = last;
-                }
-                __syncthreads();
-                const bool last = s_last != 0;
-                __syncthreads();
-                if (!last) return false;
-                // warp w: a quarter of the registers of o, for the rows that hold something
-                float mm[2] = {-INFINITY, -INFINITY}, ll[2] = {0.0f, 0.0f};
-                const bool both = cur.nr > 8;
-                for (int k = 0; k < n; ++k) {
-                    const float *src = a.part + slot_of(first + k * step) * kd_slot<HD>();
-                    mm[0] = fmaxf(mm[0], __ldcg(src + g));
-                    if (both) mm[1] = fmaxf(mm[1], __ldcg(src + g + 8));
-                }
-                float oo[NT / 4][4] = {};
-                const float base[2] = {mm[0] == -INFINITY ? 0.0f : mm[0], mm[1] == -INFINITY ? 0.0f : mm[1]};
-#pragma unroll 4
-                for (int k = 0; k < n; ++k) {
-                    const float *src = a.part + slot_of(first + k * step) * kd_slot<HD>();
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        if (r && !both) break;
-                        const float w = ex2(__ldcg(src + g + 8 * r) - base[r]);
-                        ll[r] = fmaf(w, __ldcg(src + KD_ROWS + g + 8 * r), ll[r]);
-#pragma unroll
-                        for (int i = 0; i < NT / 4; ++i)
-#pragma unroll
-                            for (int e = 2 * r; e < 2 * r + 2; ++e)
-                                oo[i][e] = fmaf(w, __ldcg(src + 2 * KD_ROWS + (4 * (warp * (NT / 4) + i) + e) * 32 + lane), oo[i][e]);
-                    }
-                }
-                // back together in warp 0
-                float *to = s_o;
+            auto part = [&](int k) { return a.part + (size_t)(k == 0 ? 2 * b0 + 1 : 2 * (b0 + k)) * kd_slot<HD>(); };
+            auto put = [&](float *to) {                   // m, l and o in fragment order, a quarter a warp
                 if (warp == 0 && t == 0) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        to[g + 8 * r] = mm[r];
-                        to[KD_ROWS + g + 8 * r] = ll[r];
+                        to[g + 8 * r] = m[r];
+                        to[KD_ROWS + g + 8 * r] = l[r];
                     }
                 }
+                to += 2 * KD_ROWS + warp * NQT * 128 + lane;
 #pragma unroll
-                for (int i = 0; i < NT / 4; ++i)
+                for (int i = 0; i < NQT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) to[2 * KD_ROWS + (4 * (warp * (NT / 4) + i) + e) * 32 + lane] = oo[i][e];
-                __syncthreads();
-                if (warp == 0) {
+                    for (int e = 0; e < 4; ++e) __stcg(to + (4 * i + e) * 32, oq[i][e]);
+            };
+            // parts first, first + step, ... (count of them): joined by the last of their blocks
+            auto join = [&](int *counter, int first, int step, int count) -> bool {
+                named_bar_sync(1, KD_WARPS * 32);
+                if (tid == 0) {
+                    __threadfence();
+                    const int last = atomicAdd(counter, 1) == count - 1;
+                    if (last) *counter = 0;               // ready for the next call
+                    __threadfence();
+                    s_last = last;
+                }
+                named_bar_sync(1, KD_WARPS * 32);
+                if (!s_last) return false;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        m[r] = to[g + 8 * r];
-                        l[r] = to[KD_ROWS + g + 8 * r];
+                for (int x = 0; x < KD_JOIN / 8; ++x) {
+                    const int k = tid / KD_ROWS + 8 * x, row = tid % KD_ROWS;
+                    if (k < count) {
+                        s_m[k * KD_ROWS + row] = __ldcg(part(first + k * step) + row);
+                        s_l[k * KD_ROWS + row] = __ldcg(part(first + k * step) + KD_ROWS + row);
+                    }
+                }
+                constexpr int F = 4;                      // parts in flight
+#pragma unroll
+                for (int i = 0; i < NQT; ++i) oq[i][0] = oq[i][1] = oq[i][2] = oq[i][3] = 0.0f;
+                for (int k0 = 0; k0 < count; k0 += F) {
+                    float v[F][NQT][4];
+#pragma unroll
+                    for (int x = 0; x < F; ++x) {
+                        const float *src = part(first + min(k0 + x, count - 1) * step) + 2 * KD_ROWS + warp * NQT * 128 + lane;
+#pragma unroll
+                        for (int i = 0; i < NQT; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[x][i][e] = e < 2 || cur.nr > 8 ? __ldcg(src + (4 * i + e) * 32) : 0.0f;
+                    }
+                    if (k0 == 0) {
+                        named_bar_sync(1, KD_WARPS * 32);
+                        common(count);
                     }
 #pragma unroll
-                    for (int i = 0; i < NT; ++i)
+                    for (int x = 0; x < F; ++x) {
+                        if (k0 + x >= count) break;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[i][e] = to[2 * KD_ROWS + (4 * i + e) * 32 + lane];
+                        for (int r = 0; r < 2; ++r) {
+                            const float w = m[r] == -INFINITY ? 0.0f : ex2(s_m[(k0 + x) * KD_ROWS + g + 8 * r] - m[r]);
+#pragma unroll
+                            for (int i = 0; i < NQT; ++i)
+#pragma unroll
+                                for (int e = 2 * r; e < 2 * r + 2; ++e) oq[i][e] = fmaf(w, v[x][i][e], oq[i][e]);
+                        }
+                    }
                 }
                 return true;
             };
-            int *const groups = a.counters, *const items = a.counters + 2 * KD_MAX_GRID;
-            if (join(groups + slot_of(gi * gs), n_in, gi * gs, 1, n_in)) {
-                if (ng == 1) write = true;
-                else {
-                    if (warp == 0) put(a.part + slot_of(gi * gs) * kd_slot<HD>());
-                    write = join(items + b0, ng, 0, gs, ng);
-                }
+            put(part(p));
+            write = join(a.counters + (gi == 0 ? 2 * b0 + 1 : 2 * (b0 + gi * gs)), gi * gs, 1, n_in);
+            if (write && ng > 1) {
+                put(part(gi * gs));
+                write = join(a.counters + 2 * KD_MAX_GRID + b0, 0, gs, ng);
             }
         }
-        if (write && warp == 0) {
+        if (write) {
             const int kh = cur.head(a);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -632,31 +839,30 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 2) k_kv_attend(const __grid_con
                 const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
                 if constexpr (!F32C) {
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const float v[2] = {o[i][2 * r] * inv, o[i][2 * r + 1] * inv};
-                        if constexpr (F32I) *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t) = make_float2(v[0], v[1]);
+                    for (int i = 0; i < NQT; ++i) {
+                        const float v[2] = {oq[i][2 * r] * inv, oq[i][2 * r + 1] * inv};
+                        TI *to = dst + 8 * (warp * NQT + i) + 2 * t;
+                        if constexpr (F32I) *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
                         else {
                             uint32_t w[1];
                             split_pair<HALF, 1>(v[0], v[1], w);
-                            *reinterpret_cast<uint32_t *>(dst + 8 * i + 2 * t) = w[0];
+                            *reinterpret_cast<uint32_t *>(to) = w[0];
                         }
                     }
-                } else {
+                } else {                                  // n tile 4cb + x, column n: 32cb + 4n + x
+                    const int n0 = warp * NQT;
 #pragma unroll
-                    for (int cb = 0; cb < HD / 32; ++cb)
+                    for (int i = 0; i < NQT; i += 2)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            *reinterpret_cast<float4 *>(dst + 32 * cb + 8 * t + 4 * e) =
-                                make_float4(o[4 * cb][2 * r + e] * inv, o[4 * cb + 1][2 * r + e] * inv,
-                                            o[4 * cb + 2][2 * r + e] * inv, o[4 * cb + 3][2 * r + e] * inv);
+                            *reinterpret_cast<float2 *>(dst + 32 * ((n0 + i) / 4) + 8 * t + 4 * e + (n0 + i) % 4) =
+                                make_float2(oq[i][2 * r + e] * inv, oq[i + 1][2 * r + e] * inv);
                 }
             }
         }
-        __syncthreads();                                  // s_o and s_last are free again
-        fresh = true;
-        if (u + 1 < u1) cur.next(a, G);
+        named_bar_sync(1, KD_WARPS * 32);                 // the joining buffers are free again
+        if (u < u1) cur.next_item(a, G);
     }
-    cp_async_wait_all();
 }
 
 // Workspace: counters, then the parts.
@@ -668,7 +874,7 @@ size_t kv_attend_ws_bytes(int hd, int type) {
 }
 
 template <typename TI, typename TC, int HD>
-static int launch_kd(const AttendArgs &a, cudaStream_t s) {
+static int launch_kd(const AttendArgs &a, const CUtensorMap *maps, cudaStream_t s) {
     static std::atomic<bool> set[64];                    // once per device
     int dev = 0;
     CPG_CUDA(cudaGetDevice(&dev));
@@ -678,24 +884,26 @@ static int launch_kd(const AttendArgs &a, cudaStream_t s) {
         if (dev < 64) set[dev].store(true, std::memory_order_release);
     }
     const int grid = std::min(KD_MAX_GRID, 2 * sm_count());
-    const cudaError_t ce = launch_pdl(k_kv_attend<TI, TC, HD>, dim3(grid), dim3(KD_WARPS * 32), (size_t)kd_smem<HD>(), s, a);
+    const cudaError_t ce = launch_pdl(k_kv_attend<TI, TC, HD>, dim3(grid), dim3(KD_THREADS), (size_t)kd_smem<HD>(), s, a,
+                                      maps[0], maps[1]);
     return ce == cudaSuccess ? CPG_OK : cuda_fail(ce, "cpg_kv_attend");
 }
 template <typename TI, typename TC>
-static int launch_hd(int hd, const AttendArgs &a, cudaStream_t s) {
-    return hd == 128 ? launch_kd<TI, TC, 128>(a, s) : launch_kd<TI, TC, 64>(a, s);
+static int launch_hd(int hd, const AttendArgs &a, const CUtensorMap *maps, cudaStream_t s) {
+    return hd == 128 ? launch_kd<TI, TC, 128>(a, maps, s) : launch_kd<TI, TC, 64>(a, maps, s);
 }
 
-int kv_attend_launch(const KvView &c, int hd, const KvRows &b, const void *q, size_t q_stride, void *out,
-                     size_t out_stride, int type, int n_heads, float scale, int window, int max_new, void *ws,
+int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &b, const void *q, size_t q_stride,
+                     void *out, size_t out_stride, int type, int n_heads, float scale, int window, int max_new, void *ws,
                      cudaStream_t s) {
     const AttendArgs a{b, c, q, out, q_stride, out_stride, n_heads, scale * 1.4426950408889634f, window,
-                       (float *)((uint8_t *)ws + KD_COUNTERS), (int *)ws};
+                       std::min(maps.box, KD_TILE), (float *)((uint8_t *)ws + KD_COUNTERS), (int *)ws};
+    const CUtensorMap *m = maps.m;
     if (type == CPG_T_F32)
-        return c.type == CPG_T_F32   ? launch_hd<float, float>(hd, a, s)
-               : c.type == CPG_T_F16 ? launch_hd<float, __half>(hd, a, s)
-                                     : launch_hd<float, __nv_bfloat16>(hd, a, s);
-    return type == CPG_T_F16 ? launch_hd<__half, __half>(hd, a, s) : launch_hd<__nv_bfloat16, __nv_bfloat16>(hd, a, s);
+        return c.type == CPG_T_F32   ? launch_hd<float, float>(hd, a, m, s)
+               : c.type == CPG_T_F16 ? launch_hd<float, __half>(hd, a, m, s)
+                                     : launch_hd<float, __nv_bfloat16>(hd, a, m, s);
+    return type == CPG_T_F16 ? launch_hd<__half, __half>(hd, a, m, s) : launch_hd<__nv_bfloat16, __nv_bfloat16>(hd, a, m, s);
 }
 
 }  // namespace cpg

@@ -104,11 +104,14 @@ class KVCache:
         return stride[0] if batch.rows > 1 else t.shape[1] * self.head_dim
 
     def _call(self, stream, fn, *args):
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
+        index = self.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
                 return self._call(stream, fn, *args)
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        check(fn(self.handle, *args, s.cuda_stream))
+        s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
+        rc = fn(self.handle, *args, s)
+        if rc:
+            check(rc)
 
     def append(self, batch: KVBatch, q, k, v, *, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, stream=None):
         """Keys and values of the batch's rows into their pages; returns the queries, normed and
