@@ -32,6 +32,7 @@
 #include <vector>
 
 #include "gemm_tc.cuh"
+#include "tcgen05.cuh"
 
 namespace cpg {
 
@@ -60,80 +61,6 @@ constexpr int TC_TMEM_COLS = 2 * TC_BN;     // two fp32 accumulators of 256 colu
 constexpr int TC_MAX_E = 256;
 static_assert(TC_STAGE0 % 1024 == 0 && TC_STAGE_BYTES % 1024 == 0 && TC_A_BYTES % 1024 == 0,
               "operand tiles must stay 1024-byte aligned");
-
-// ---------------------------------------------------------------- tcgen05 / TMA wrappers
-// SM100 shared-memory matrix descriptor, K-major, no swizzle: start, LBO, SBO in 16-byte units,
-// version 1 (bit 46), base offset 0, layout type 0.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
-}
-
-// K-major, 64-byte swizzle (the layout a SWIZZLE_64B tensor TMA writes): rows of 64 bytes,
-// 8-row groups 512 bytes apart (SBO), LBO unused (1), layout type 4. Advancing K by 16 fp16
-// values inside the 64-byte row moves the start address by 32 bytes.
-__device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(512 >> 4) << 32) | (1ull << 46) |
-           (4ull << 61);
-}
-
-// kind::f16 instruction descriptor: fp32 accumulate, fp16 A and B, both K-major, M, N.
-__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
-    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// 2D tensor TMA load (no multicast) of the box at (x, y) into shared memory, completing on bar.
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
-// 32 consecutive fp32 columns of this warp's 32 TMEM lanes.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Bounded wait that also honours the CTA-wide abort flag.
-__device__ __forceinline__ bool tc_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status,
-                                        int code) {
-    if (*abort_flag) return false;
-    if (mbar_wait(bar, parity)) return true;
-    *abort_flag = 1;
-    atomicCAS(status, ST_OK, code);
-    return false;
-}
 
 // Q4_0 group pair (36 bytes as 9 words: scale d0 + 16 quant bytes, scale d1 + 16 quant bytes)
 // -> 64 fp16 values q*d in K order, as 8 chunks of 8 values (16 bytes each).

@@ -41,28 +41,10 @@
 #include <atomic>
 #include <type_traits>
 
-#include "kv.cuh"
+#include "kv_attend.cuh"
 
 namespace cpg {
 
-struct AttendArgs {
-    KvRows b;
-    KvView c;
-    const void *q;
-    void *out;
-    size_t q_stride, out_stride;
-    int H;
-    float scale2;                    // scale · log2(e)
-    int window, box;                 // box: positions of one tensor TMA load
-    float *part;                     // 2 slots per block
-    int *counters;                   // 2 per block (groups, by slot), then 1 per block (items)
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -88,19 +70,6 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-// 4D tensor TMA load (no multicast) of the box at (x, place, head, page).
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int place, int head, int page,
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(place), "r"(head), "r"(page), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
 // d += a·b, m16n8k16, of f16 (HALF) or bf16 operands.
 template <bool HALF>
 __device__ __forceinline__ void mma_acc(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -114,57 +83,15 @@ __device__ __forceinline__ void mma_acc(float (&d)[4], const uint32_t (&a)[4], u
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// (x, y) as N terms of two 16-bit halves each, largest first. f16: rounded, 22 bits from two terms.
-// bf16: one term rounded; three terms cut off, which leaves nothing of an f32.
-template <bool HALF, int N>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[N]) {
-    if constexpr (HALF) {
-        const __half2 h = __floats2half2_rn(x, y);
-        t[0] = *reinterpret_cast<const uint32_t *>(&h);
-        if constexpr (N == 2) {
-            const float2 f = __half22float2(h);
-            const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-            t[1] = *reinterpret_cast<const uint32_t *>(&l);
-        }
-    } else if constexpr (N == 1) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        t[0] = *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-            t[i] = __byte_perm(a, b, 0x7632);
-            x -= __uint_as_float(a & 0xffff0000u);
-            y -= __uint_as_float(b & 0xffff0000u);
-        }
-    }
-}
-
 constexpr int KD_WARPS = 4, KD_KEYS = 16, KD_TILE = KD_WARPS * KD_KEYS, KD_ROWS = 16;
 constexpr int KD_THREADS = (KD_WARPS + 1) * 32;
 constexpr int KD_RING = 96 * 1024;
-constexpr int KD_MAX_GRID = 512;
 template <int HD> constexpr int kd_slot() { return 2 * KD_ROWS + HD / 2 * 32; }   // floats: m, l, o in fragment order
-constexpr int KD_JOIN = 24;                              // parts of one join, at most (root of KD_MAX_GRID)
+constexpr int KD_JOIN = 24;                              // parts of one join, at most (root of KV_MAX_GRID)
 // behind the ring: q's terms (f32 rows) and later three quarters of half the warps' sums, both
 // 3 · HD / 16 · 512 bytes; the maxima and sums of what is joined
 template <int HD> constexpr int kd_buf() { return 3 * HD / 16 * 512; }
 template <int HD> constexpr int kd_smem() { return 1008 + KD_RING + kd_buf<HD>() + KD_JOIN * 2 * KD_ROWS * 4; }
-
-// a / b of non-negative numbers; nearly always both have 32 bits, which divide in a fifth of the time.
-__device__ __forceinline__ long kd_div(long a, long b) {
-    return ((a | b) >> 32) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-// Units 0..U-1 over NB blocks: block b has [start(b), start(b + 1)), the first U % NB one more.
-struct KdCut {
-    long each, more;
-    __device__ __forceinline__ KdCut(long U, long NB) : each(kd_div(U, NB)), more(U - each * NB) {}
-    __device__ __forceinline__ long start(long b) const { return b * each + min(b, more); }
-    __device__ __forceinline__ int owner(long u) const {
-        const long big = more * (each + 1);
-        return (int)(u < big ? kd_div(u, each + 1) : more + kd_div(u - big, each));
-    }
-};
 
 // Sequence i's units: KV · row tiles · (KD_FIXED + position tiles), the same for each of its items.
 // Beginning and ending an item takes a block as long as some three tiles (4 us against 1.4 us for 64
@@ -253,12 +180,12 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     long U = 0, before = 0, u0 = 0, u1 = 0;
     int NB = 0;
     const int blk = blockIdx.x;
-    KdCut cut(0, 1);
+    KvCut cut(0, 1);
     auto range = [&](long total) {                        // false: nothing for this block
         U = total;
         NB = (int)min((long)gridDim.x, U);
         if (blk >= NB) return false;
-        cut = KdCut(U, NB);
+        cut = KvCut(U, NB);
         u0 = cut.start(blk);
         u1 = cut.start(blk + 1);
         return true;
@@ -311,7 +238,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     KdCursor cur;
     cur.seq = s_seq;
     cur.q = s_item;
-    cur.sub = (int)kd_div(s_off, cur.q.nt + KD_FIXED);
+    cur.sub = (int)kv_div(s_off, cur.q.nt + KD_FIXED);
     cur.kt = (int)(s_off - (long)cur.sub * (cur.q.nt + KD_FIXED)) - KD_FIXED;
     cur.item(a, G);
     volatile int *const abort_flag = &s_abort;
@@ -321,6 +248,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         const int groups = KD_TILE / a.box;
         const uint32_t ring = smem_u32(smem);
         int slot = 0, turn = 0;
+        bool stop = false;
         for (long u = u0; u < u1; ++u) {
             if (cur.kt < 0) {                             // nothing to load
                 ++cur.kt;
@@ -344,11 +272,13 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {        // K, then V
-                if (turn && !mbar_wait(&empty[slot], (uint32_t)(turn - 1) & 1u)) {
+                const bool ok = !turn || *abort_flag || mbar_wait(&empty[slot], (uint32_t)(turn - 1) & 1u);
+                if (!ok) {
                     *abort_flag = 1;
                     atomicOr(a.c.status, KV_TIMEOUT);
                 }
-                if (*abort_flag) break;
+                stop = __any_sync(0xffffffffu, !ok || *abort_flag);
+                if (stop) break;
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
                 __syncwarp();
 #pragma unroll
@@ -363,10 +293,10 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                     ++turn;
                 }
             }
-            if (*abort_flag) break;
+            if (stop) break;
             if (++cur.kt == cur.q.nt && u + 1 < u1) cur.next_item(a, G);
         }
-        if (*abort_flag) {                                // copies in flight land before the block may end
+        if (stop) {                                       // copies in flight land before the block may end
             for (int i = 0; i < NU; ++i) {
                 const int n = turn + (i < slot);          // fills of slot i
                 if (n) mbar_wait(&full[i], (uint32_t)(n - 1) & 1u);
@@ -826,7 +756,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             write = join(a.counters + (gi == 0 ? 2 * b0 + 1 : 2 * (b0 + gi * gs)), gi * gs, 1, n_in);
             if (write && ng > 1) {
                 put(part(gi * gs));
-                write = join(a.counters + 2 * KD_MAX_GRID + b0, 0, gs, ng);
+                write = join(a.counters + 2 * KV_MAX_GRID + b0, 0, gs, ng);
             }
         }
         if (write) {
@@ -865,12 +795,19 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     }
 }
 
-// Workspace: counters, then the parts.
-constexpr size_t KD_COUNTERS = (3 * KD_MAX_GRID * sizeof(int) + 255) / 256 * 256;
+int kv_attend_tc_launch(const AttendArgs &a, const CUtensorMap *maps, int hd, cudaStream_t s);
+size_t kv_attend_tc_part_bytes(int hd);
+
+// Workspace: counters (of this kernel, then of the chunk kernel's), then the parts. The counters
+// lie at fixed places and are zero between calls, so calls of any shape may follow one another.
+constexpr size_t KD_COUNTERS = 3 * KV_MAX_GRID, KT_COUNTERS = 6 * KV_MAX_GRID;
+constexpr size_t KV_PARTS_AT = (KD_COUNTERS + KT_COUNTERS) * sizeof(int);
+static_assert(KV_PARTS_AT % 256 == 0, "parts start at a 256-byte boundary");
 
 size_t kv_attend_ws_bytes(int hd, int type) {
     const size_t slot = (hd == 128 ? kd_slot<128>() : kd_slot<64>()) * sizeof(float);
-    return KD_COUNTERS + 2 * (size_t)KD_MAX_GRID * slot;
+    const size_t parts = 2 * (size_t)KV_MAX_GRID * slot;
+    return KV_PARTS_AT + (type == CPG_T_F32 ? parts : std::max(parts, kv_attend_tc_part_bytes(hd)));
 }
 
 template <typename TI, typename TC, int HD>
@@ -883,7 +820,7 @@ static int launch_kd(const AttendArgs &a, const CUtensorMap *maps, cudaStream_t 
         if (rc) return rc;
         if (dev < 64) set[dev].store(true, std::memory_order_release);
     }
-    const int grid = std::min(KD_MAX_GRID, 2 * sm_count());
+    const int grid = std::min(KV_MAX_GRID, 2 * sm_count());
     const cudaError_t ce = launch_pdl(k_kv_attend<TI, TC, HD>, dim3(grid), dim3(KD_THREADS), (size_t)kd_smem<HD>(), s, a,
                                       maps[0], maps[1]);
     return ce == cudaSuccess ? CPG_OK : cuda_fail(ce, "cpg_kv_attend");
@@ -896,9 +833,18 @@ static int launch_hd(int hd, const AttendArgs &a, const CUtensorMap *maps, cudaS
 int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &b, const void *q, size_t q_stride,
                      void *out, size_t out_stride, int type, int n_heads, float scale, int window, int max_new, void *ws,
                      cudaStream_t s) {
-    const AttendArgs a{b, c, q, out, q_stride, out_stride, n_heads, scale * 1.4426950408889634f, window,
-                       std::min(maps.box, KD_TILE), (float *)((uint8_t *)ws + KD_COUNTERS), (int *)ws};
+    AttendArgs a{b, c, q, out, q_stride, out_stride, n_heads, scale * 1.4426950408889634f, window, maps.box,
+                 (float *)((uint8_t *)ws + KV_PARTS_AT), (int *)ws};
     const CUtensorMap *m = maps.m;
+    // Rows of a sequence and cached head past one row tile of this file's kernel go to the chunk
+    // kernel: its 2 x 128 rows share each tile of K and V that is read.
+    const int G = n_heads / c.KV;
+    const long most = max_new > 0 ? std::min(max_new, b.T) : b.T;
+    if (type != CPG_T_F32 && G <= 128 && most * G > KD_ROWS) {
+        a.counters += KD_COUNTERS;
+        return kv_attend_tc_launch(a, m, hd, s);
+    }
+    a.box = std::min(maps.box, KD_TILE);
     if (type == CPG_T_F32)
         return c.type == CPG_T_F32   ? launch_hd<float, float>(hd, a, m, s)
                : c.type == CPG_T_F16 ? launch_hd<float, __half>(hd, a, m, s)
