@@ -3,7 +3,9 @@
 // The reference keeps one contiguous f32 cache per sequence (qwen3_moe.h:40-70); here the
 // positions of many sequences share pools of fixed-size pages, found through a table per sequence.
 #include <math.h>
+#include <stddef.h>
 
+#include <algorithm>
 #include <new>
 
 #include "kv.cuh"
@@ -13,13 +15,21 @@ struct cpg_kv {
     cpg::KvMaps maps;
     int hd, device, rope_dim, rope_f32;
     float theta;
-    double freq[64];                 // theta^(-2j/R) / pi: a position's angle in half turns is p·freq
+    bool owns;                       // the device block is this handle's (kv_create_like shares it)
+};
+
+// The handle's device memory: the status word, and theta^(-2j/R) / pi (a position's angle in half
+// turns is p times that). Device memory, not a launch argument: lanes that index the constant bank
+// with different j are served one after another.
+struct KvDevice {
+    int status, pad[31];
+    double freq[64];
 };
 
 namespace cpg {
 
 // ------------------------------------------------------------------------------ append
-// One block per row (and per group of heads, for few rows). For every query and key head x:
+// One block per run of rows, or for few rows one per row and group of heads. For every query and key head x:
 // y = x / sqrt(mean x² + eps) · g (head_rmsnorm, qwen3_moe.c:44-49; only with a gain), then the
 // rotation of (y_j, y_{j+R/2}) by p·theta^(-2j/R) (rope_apply_from, kernels.c:425-447). Queries go
 // to q_out, keys and values to the row's place in the pools, each value rounded once.
@@ -29,9 +39,16 @@ namespace cpg {
 // exact, and the rest in [-1, 1] goes to sincospif. With rope_f32 it is the reference's arithmetic
 // instead: an f32 frequency, an f32 product.
 //
-// A thread holds 16 bytes of a head; lanes of a head exchange rotation partners by shuffle (R/2 is
-// a multiple of a thread's elements). The row's R/2 sines are computed once per block while the
-// first heads' loads are in flight.
+// HD / 8 threads hold a head, each two groups of four elements that are rotation partners (elements
+// 4c.. and R/2 + 4c.., c < R / 8; the rest in pairs of neighbours), so nothing crosses lanes but the
+// sum of squares, and a row's sines are the same registers for all of a thread's heads. The rows'
+// places (a search over q_start, then the table) and sines are found once per block, while the first
+// row's loads are in flight.
+//
+// Bound by memory: each value is read and written once. What counts is the bytes in flight, so a
+// thread asks for the next row's heads, unconverted, before it works on this one's (without that
+// 16384 rows of 32 + 2·4 heads in bf16 took 111 us instead of 85), and
+// a run is as long as one wave of blocks needs to take all rows.
 struct AppendArgs {
     KvRows b;
     KvView c;
@@ -40,138 +57,190 @@ struct AppendArgs {
     size_t q_stride, k_stride, v_stride, qo_stride;
     const float *q_norm, *k_norm;
     float eps, theta;
-    int H, R, rope_f32;
-    double freq[64];
+    int H, R, rope_f32, rows;
+    const double *freq;
 };
 
-constexpr int AP_U = 4;              // heads of a lane group in flight
+constexpr int AP_U = 4, AP_MAX_ROWS = 32, AP_BLOCKS = 4;   // query heads of a lane group in flight; rows of a block; blocks per SM
+
+// Four elements as they lie in memory, and as f32.
+template <typename T> struct Quad;
+template <> struct Quad<float> { using type = float4; };
+template <> struct Quad<__half> { using type = uint2; };
+template <> struct Quad<__nv_bfloat16> { using type = uint2; };
 
 template <typename TI, typename TC, int HD>
-__global__ void __launch_bounds__(512) k_kv_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_constant__ AppendArgs a) {
+    using Raw = typename Quad<TI>::type;
     pdl_wait();
     pdl_launch_dependents();
-    constexpr int N = 16 / (int)sizeof(TI);               // elements per thread
-    constexpr int LPH = HD / N, HPW = 32 / LPH;           // lanes per head, heads per warp
-    __shared__ float2 s_cs[64];
-    __shared__ int s_where[3];                            // position, page, live
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-    const int KV = a.c.KV, nh = a.H + 2 * KV;             // heads q, then k, then v
-    const int sub = lane % LPH, e0 = sub * N;
-    const int groups = (blockDim.x >> 5) * HPW;           // heads of the block in flight
-    const int per = (nh + gridDim.y - 1) / gridDim.y;     // this block's heads
-    const int h0 = blockIdx.y * per, h1 = min(nh, h0 + per);
-    const int first = h0 + (tid >> 5) * HPW + lane / LPH;
+    constexpr int TPH = HD / 8, HPW = 32 / TPH;           // threads per head, heads per warp
+    extern __shared__ float2 s_cs[];                      // (rows, R / 2)
+    __shared__ int s_pos[AP_MAX_ROWS], s_page[AP_MAX_ROWS];   // position, -1: no sequence's row; page, -1: none
+    const int t0 = blockIdx.x * a.rows, rows = min(a.rows, a.b.T - t0);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int KV = a.c.KV, R = a.R;
+    const int sub = lane % TPH;
+    const bool turns = sub < R / 8;
+    const int ea = turns ? 4 * sub : 8 * sub, eb = ea + (turns ? R / 2 : 4);   // 8·sub = R + 8·(sub - R/8)
+    // lane groups of a row, over all its blocks: group `grp` takes the heads grp, grp + groups, ...
+    const int groups = gridDim.y * (blockDim.x >> 5) * HPW;
+    const int grp = (blockIdx.y * (blockDim.x >> 5) + warp) * HPW + lane / TPH;
 
-    float x[AP_U][N];
-    auto load = [&](int base) {
+    // a row's query heads from h, and its key or value head h
+    auto load_q = [&](Raw (&x)[AP_U][2], int t, int h) {
+        const TI *src = (const TI *)a.q + (size_t)t * a.q_stride + h * HD;
 #pragma unroll
-        for (int u = 0; u < AP_U; ++u) {
-            const int h = base + u * groups;
-            if (h >= h1) continue;
-            const TI *src = h < a.H ? (const TI *)a.q + (size_t)t * a.q_stride + (size_t)h * HD
-                            : h < a.H + KV ? (const TI *)a.k + (size_t)t * a.k_stride + (size_t)(h - a.H) * HD
-                                           : (const TI *)a.v + (size_t)t * a.v_stride + (size_t)(h - a.H - KV) * HD;
-            load_vec<TI, N>(src + e0, x[u]);
-        }
+        for (int u = 0; u < AP_U; ++u)
+            if (h + u * groups < a.H) {
+                x[u][0] = *reinterpret_cast<const Raw *>(src + u * groups * HD + ea);
+                x[u][1] = *reinterpret_cast<const Raw *>(src + u * groups * HD + eb);
+            }
     };
-    load(first);
+    auto load_kv = [&](Raw (&x)[2], int t, int h) {
+        if (h >= 2 * KV) return;
+        const TI *src = (h < KV ? (const TI *)a.k + (size_t)t * a.k_stride : (const TI *)a.v + (size_t)t * a.v_stride) +
+                        (h < KV ? h : h - KV) * HD;
+        x[0] = *reinterpret_cast<const Raw *>(src + ea);
+        x[1] = *reinterpret_cast<const Raw *>(src + eb);
+    };
+    Raw nq[AP_U][2], nkv[2];                              // the next row's
+    load_q(nq, t0, grp);
+    load_kv(nkv, t0, grp);
 
-    if (tid < 32) {
-        const int i = kv_find_seq(a.b.q_start, a.b.n, t);
-        int pos = 0, page = -1, live = 0;
+    for (int r = warp; r < rows; r += blockDim.x >> 5) {
+        const int t = t0 + r, i = kv_find_seq(a.b.q_start, a.b.n, t);
+        int pos = -1, page = -1;
         if (i < a.b.n) {
             const int a0 = a.b.q_start[i], p0 = a.b.pos0[i];
             if (t >= a0 && p0 >= 0) {
-                live = 1;
                 const long p = (long)p0 + (t - a0);
                 pos = (int)min(p, 0x7fffffffl);
-                const long at = p / a.c.P;
-                if (at < a.b.max_pages) page = a.b.pages[(size_t)i * a.b.table_stride + at];
+                const int at = pos / a.c.P;
+                const bool inside = p <= 0x7fffffffl && at < a.b.max_pages;
+                if (inside) page = a.b.pages[(size_t)i * a.b.table_stride + at];
                 if (page < 0 || page >= a.c.n_pages) {
                     page = -1;
-                    if (lane == 0) atomicOr(a.c.status, at < a.b.max_pages ? KV_BAD_PAGE : KV_BAD_POS);
+                    if (lane == 0) atomicOr(a.c.status, inside ? KV_BAD_PAGE : KV_BAD_POS);
                 }
             } else if (lane == 0 && p0 < 0) {
                 atomicOr(a.c.status, KV_BAD_POS);
             }
         }
         if (lane == 0) {
-            s_where[0] = pos;
-            s_where[1] = page;
-            s_where[2] = live;
+            s_pos[r] = pos;
+            s_page[r] = page;
         }
     }
+    float gq[8];
+    if (a.q_norm) {
+        load4(a.q_norm + ea, gq);
+        load4(a.q_norm + eb, gq + 4);
+    }
     __syncthreads();
-    if (!s_where[2]) return;                              // a row of no sequence
-    const int pos = s_where[0], page = s_where[1], R = a.R;
-    for (int j = tid; j < R / 2; j += blockDim.x) {
+    for (int z = tid; z < rows * (R / 2); z += blockDim.x) {
+        const int r = z / (R / 2), j = z - r * (R / 2), pos = s_pos[r];
         float sn, cs;
         if (a.rope_f32) {
             const float ang = __fmul_rn((float)pos, powf(a.theta, __fdiv_rn(-2.0f * (float)j, (float)R)));
             cs = cosf(ang);
             sn = sinf(ang);
         } else {
-            const double turn = (double)pos * a.freq[j];
+            const double turn = (double)pos * __ldg(a.freq + j);
             sincospif((float)(turn - 2.0 * rint(0.5 * turn)), &sn, &cs);
         }
-        s_cs[j] = make_float2(cs, sn);
+        s_cs[z] = make_float2(cs, sn);
     }
     __syncthreads();
-    const size_t place = page < 0 ? 0 : (size_t)page * a.c.sp + (size_t)(pos % a.c.P) * a.c.st + e0;
+    // the sums below are among the threads of one head, which agree on everything that branches
+    const unsigned mask = ((1u << TPH) - 1u) << (lane / TPH * TPH);
 
-    for (int base = first; base < h1; base += AP_U * groups) {
-        if (base != first) load(base);
+    auto norm = [&](float (&y)[8], const float (&g)[8]) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+#pragma unroll
+        for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const float inv = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= inv * g[i];
+    };
+    for (int r = 0; r < rows; ++r) {
+        const int t = t0 + r, pos = s_pos[r], page = s_page[r];
+        Raw xq[AP_U][2], xkv[2];
 #pragma unroll
         for (int u = 0; u < AP_U; ++u) {
-            const int h = base + u * groups;
-            // the shuffles below are among the lanes of one head, which agree on h
-            const unsigned mask = LPH == 32 ? 0xffffffffu : (((1u << (LPH & 31)) - 1u) << (lane / LPH * LPH));
-            if (h >= h1) continue;
-            float(&y)[N] = x[u];
-            if (h < a.H + KV) {
-                const float *gain = h < a.H ? a.q_norm : a.k_norm;
-                if (gain) {
-                    float ss = 0.0f;
+            xq[u][0] = nq[u][0];
+            xq[u][1] = nq[u][1];
+        }
+        xkv[0] = nkv[0];
+        xkv[1] = nkv[1];
+        if (r + 1 < rows) {
+            load_q(nq, t + 1, grp);
+            load_kv(nkv, t + 1, grp);
+        }
+        if (pos < 0) continue;                            // a row of no sequence
+        float2 cs[4] = {};
+        if (turns) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) ss = fmaf(y[i], y[i], ss);
+            for (int i = 0; i < 4; ++i) cs[i] = s_cs[r * (R / 2) + 4 * sub + i];
+        }
+        auto turn = [&](float (&y)[8]) {
+            if (!turns) return;
 #pragma unroll
-                    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-                    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)HD) + a.eps));
-                    float g[N];
-                    load_vec<float, N>(gain + e0, g);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], inv), g[i]);
-                }
-                if (R) {
-                    const int half = R / 2, d = half / N;                // lanes to the partner
-                    const bool low = e0 < half, in = e0 < R;
-                    const int from = in ? (low ? lane + d : lane - d) : lane;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float other = __shfl_sync(mask, y[i], from);
-                        if (in) {
-                            const float2 cs = s_cs[(low ? e0 : e0 - half) + i];
-                            y[i] = low ? __fsub_rn(__fmul_rn(y[i], cs.x), __fmul_rn(other, cs.y))
-                                       : __fadd_rn(__fmul_rn(y[i], cs.x), __fmul_rn(other, cs.y));
-                        }
-                    }
-                }
+            for (int i = 0; i < 4; ++i) {
+                const float lo = y[i], hi = y[4 + i];
+                y[i] = fmaf(lo, cs[i].x, -(hi * cs[i].y));
+                y[4 + i] = fmaf(hi, cs[i].x, lo * cs[i].y);
             }
-            if (h < a.H)
-                store_vec<TI, N>((TI *)a.q_out + (size_t)t * a.qo_stride + (size_t)h * HD + e0, y);
-            else if (page >= 0) {
-                const bool isk = h < a.H + KV;
-                TC *dst = (TC *)(isk ? a.c.k : a.c.v) + place + (size_t)(h - a.H - (isk ? 0 : KV)) * a.c.sh;
-                store_vec<TC, N>(dst, y);
+        };
+        for (int h = grp;;) {
+            TI *dst = (TI *)a.q_out + (size_t)t * a.qo_stride + h * HD;
+#pragma unroll
+            for (int u = 0; u < AP_U; ++u)
+                if (h + u * groups < a.H) {
+                    float y[8];
+                    load4(reinterpret_cast<const TI *>(&xq[u][0]), y);
+                    load4(reinterpret_cast<const TI *>(&xq[u][1]), y + 4);
+                    if (a.q_norm) norm(y, gq);
+                    turn(y);
+                    store4(dst + u * groups * HD + ea, y);
+                    store4(dst + u * groups * HD + eb, y + 4);
+                }
+            h += AP_U * groups;
+            if (h >= a.H) break;
+            load_q(xq, t, h);
+        }
+        if (page < 0) continue;
+        const size_t place = (size_t)page * a.c.sp + (size_t)(pos % a.c.P) * a.c.st;
+        for (int h = grp; h < 2 * KV;) {                  // keys, then values
+            const bool isk = h < KV;
+            float y[8];
+            load4(reinterpret_cast<const TI *>(&xkv[0]), y);
+            load4(reinterpret_cast<const TI *>(&xkv[1]), y + 4);
+            if (isk) {
+                if (a.k_norm) {
+                    float gk[8];
+                    load4(a.k_norm + ea, gk);
+                    load4(a.k_norm + eb, gk + 4);
+                    norm(y, gk);
+                }
+                turn(y);
             }
+            TC *to = (TC *)(isk ? a.c.k : a.c.v) + place + (size_t)(isk ? h : h - KV) * a.c.sh;
+            store4(to + ea, y);
+            store4(to + eb, y + 4);
+            h += groups;
+            load_kv(xkv, t, h);
         }
     }
 }
 
 template <typename TI, typename TC>
 static cudaError_t launch_append(int hd, const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
-    return hd == 128 ? launch_pdl(k_kv_append<TI, TC, 128>, grid, block, 0, s, a)
-                     : launch_pdl(k_kv_append<TI, TC, 64>, grid, block, 0, s, a);
+    const size_t smem = (size_t)a.rows * (a.R / 2) * sizeof(float2);
+    return hd == 128 ? launch_pdl(k_kv_append<TI, TC, 128>, grid, block, smem, s, a)
+                     : launch_pdl(k_kv_append<TI, TC, 64>, grid, block, smem, s, a);
 }
 
 int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &b, const void *q, size_t q_stride,
@@ -188,7 +257,9 @@ static bool type_ok(int type) { return type == CPG_T_F32 || type == CPG_T_F16 ||
 
 using namespace cpg;
 
-extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) {
+// A handle of `d`; with `like`, one that shares the device block (status word, frequencies) of a
+// handle with the same rotation: the layers of a model report through one word.
+static int kv_create(const cpg_kv_desc *d, const cpg_kv *like, cpg_kv **out) {
     CPG_REQUIRE(d && out, "cpg_kv_create: null argument");
     *out = nullptr;
     CPG_REQUIRE(d->head_dim == 64 || d->head_dim == 128, "cpg_kv_create: head_dim %d (64 or 128)", d->head_dim);
@@ -231,8 +302,9 @@ extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) {
     kv->rope_dim = d->rope_dim;
     kv->rope_f32 = d->rope_f32 != 0;
     kv->theta = d->rope_theta;
+    KvDevice dev{};
     for (int j = 0; j < d->rope_dim / 2; ++j)
-        kv->freq[j] = pow((double)d->rope_theta, -2.0 * j / d->rope_dim) / 3.14159265358979323846;
+        dev.freq[j] = pow((double)d->rope_theta, -2.0 * j / d->rope_dim) / 3.14159265358979323846;
     kv->maps.box = 8;
     while (kv->maps.box < 64 && d->page_size % (2 * kv->maps.box) == 0) kv->maps.box *= 2;
     const uint64_t dims[4] = {hd, (uint64_t)d->page_size, (uint64_t)d->n_kv, (uint64_t)d->n_pages};
@@ -247,10 +319,12 @@ extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) {
         }
     }
     cudaError_t ce = cudaGetDevice(&kv->device);
-    if (ce == cudaSuccess) ce = cudaMalloc(&kv->v.status, sizeof(int));
-    if (ce == cudaSuccess) ce = cudaMemset(kv->v.status, 0, sizeof(int));
+    kv->owns = !like;
+    if (like) kv->v.status = like->v.status;
+    if (ce == cudaSuccess && !like) ce = cudaMalloc(&kv->v.status, sizeof(KvDevice));
+    if (ce == cudaSuccess && !like) ce = cudaMemcpy(kv->v.status, &dev, sizeof(KvDevice), cudaMemcpyHostToDevice);
     if (ce != cudaSuccess) {
-        cudaFree(kv->v.status);
+        if (kv->owns) cudaFree(kv->v.status);
         delete kv;
         return cuda_fail(ce, "cpg_kv_create");
     }
@@ -258,9 +332,14 @@ extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) {
     return CPG_OK;
 }
 
+extern "C" int cpg_kv_create(const cpg_kv_desc *d, cpg_kv **out) { return kv_create(d, nullptr, out); }
+namespace cpg {
+int kv_create_like(const cpg_kv_desc *d, const cpg_kv *like, cpg_kv **out) { return kv_create(d, like, out); }
+}  // namespace cpg
+
 extern "C" void cpg_kv_destroy(cpg_kv *kv) {
     if (!kv) return;
-    cudaFree(kv->v.status);
+    if (kv->owns) cudaFree(kv->v.status);
     delete kv;
 }
 
@@ -310,18 +389,15 @@ extern "C" int cpg_kv_append(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     a.q_norm = q_norm; a.k_norm = k_norm;
     a.eps = eps; a.theta = kv->theta;
     a.H = n_heads; a.R = kv->rope_dim; a.rope_f32 = kv->rope_f32;
-    for (int j = 0; j < a.R / 2; ++j) a.freq[j] = kv->freq[j];
-    // heads in flight per warp: 16 bytes a lane; warps for all heads of a row at AP_U each, and a
-    // row over several blocks while the rows alone leave SMs idle
-    const int per_warp = 32 * (16 / (int)type_bytes(type)) / kv->hd;
-    const int nh = n_heads + 2 * kv->v.KV;
+    a.freq = (const double *)((const char *)kv->v.status + offsetof(KvDevice, freq));
+    // Many rows: runs that one wave of AP_BLOCKS blocks per SM takes, four warps each. Few rows: one a
+    // block, and a row over several blocks while the rows alone leave SMs idle.
+    const int per_warp = 256 / kv->hd, heads = std::max(n_heads, 2 * kv->v.KV), sms = sm_count();
+    a.rows = std::min(AP_MAX_ROWS, (a.b.T + sms * AP_BLOCKS - 1) / (sms * AP_BLOCKS));
     int split = 1;
-    while (split < 8 && (long)a.b.T * split < sm_count() && nh / (split * 2) >= per_warp) split *= 2;
-    const int per = (nh + split - 1) / split;
-    int warps = (per + per_warp * AP_U - 1) / (per_warp * AP_U);
-    if (split > 1) warps = (per + per_warp - 1) / per_warp;
-    warps = warps < 2 ? 2 : warps > 16 ? 16 : warps;
-    const dim3 grid(a.b.T, split), block(32 * warps);
+    while (split < 8 && (long)a.b.T * split < sms && heads > split * 4 * per_warp) split *= 2;
+    const int warps = std::min(4, (heads + per_warp - 1) / per_warp);
+    const dim3 grid((a.b.T + a.rows - 1) / a.rows, split), block(32 * warps);
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t ce;
     if (type == CPG_T_F32)

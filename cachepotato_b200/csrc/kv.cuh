@@ -33,55 +33,31 @@ struct KvMaps {
 // Status bits a kernel leaves in KvView::status (reported and cleared by cpg_kv_check).
 enum : int { KV_BAD_PAGE = 1, KV_BAD_POS = 2, KV_TIMEOUT = 4 };
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-
-// N consecutive elements as f32 (16-byte loads where N allows) and back, each rounded once.
-template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T *p, float (&v)[N]) {
-    constexpr int B = N * (int)sizeof(T);
-    static_assert(B == 8 || B % 16 == 0, "vector width");
-    if constexpr (B == 8) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-        const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_f32(e[i]);
-    } else {
-#pragma unroll
-        for (int b = 0; b < B / 16; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p) + 16 * b);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int i = 0; i < 16 / (int)sizeof(T); ++i) v[b * (16 / sizeof(T)) + i] = to_f32(e[i]);
-        }
-    }
+// Four consecutive elements as f32, and back, each rounded once.
+__device__ __forceinline__ void load4(const float *p, float *v) {
+    const float4 w = *reinterpret_cast<const float4 *>(p);
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_vec(T *p, const float (&v)[N]) {
-    constexpr int B = N * (int)sizeof(T);
-    static_assert(B == 8 || B % 16 == 0, "vector width");
-    if constexpr (B == 8) {
-        uint2 w;
-        T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = from_f32<T>(v[i]);
-        *reinterpret_cast<uint2 *>(p) = w;
-    } else {
-#pragma unroll
-        for (int b = 0; b < B / 16; ++b) {
-            uint4 w;
-            T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-            for (int i = 0; i < 16 / (int)sizeof(T); ++i) e[i] = from_f32<T>(v[b * (16 / sizeof(T)) + i]);
-            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p) + 16 * b) = w;
-        }
-    }
+__device__ __forceinline__ void load4(const __half *p, float *v) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float *v) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float *p, const float *v) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__half *p, const float *v) {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
 
 // The number of entries of q_start[1..n] that are <= t: the sequence row t belongs to where the
