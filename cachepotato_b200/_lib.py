@@ -37,6 +37,8 @@ EXPORTS = [
     "cpg_qwen3_batch_generate", "cpg_qwen3_batch_position", "cpg_qwen3_batch_logits",
     "cpg_kv_create", "cpg_kv_destroy", "cpg_kv_append", "cpg_kv_attend", "cpg_kv_attend_workspace_bytes",
     "cpg_kv_check",
+    "cpg_qwen3_paged_create", "cpg_qwen3_paged_destroy", "cpg_qwen3_paged_step", "cpg_qwen3_paged_generate",
+    "cpg_qwen3_paged_drop", "cpg_qwen3_paged_position", "cpg_qwen3_paged_free_pages", "cpg_qwen3_paged_logits",
 ]
 
 
@@ -162,6 +164,14 @@ _SIGS = {
     "cpg_kv_attend_workspace_bytes": (_sz, [_vp, _i]),
     "cpg_kv_attend": (_i, [_vp, ctypes.POINTER(KvRows), _i, _i, _vp, _l, _vp, _l, _f, _i, _vp, _sz, _vp]),
     "cpg_kv_check": (_i, [_vp, _vp]),
+    "cpg_qwen3_paged_create": (_i, [_vp, _i, _i, _i, _i, _i, ctypes.POINTER(_vp)]),
+    "cpg_qwen3_paged_destroy": (None, [_vp]),
+    "cpg_qwen3_paged_step": (_i, [_vp, _vp, _vp, _vp, _i, _vp]),
+    "cpg_qwen3_paged_generate": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
+    "cpg_qwen3_paged_drop": (_i, [_vp, _i]),
+    "cpg_qwen3_paged_position": (_i, [_vp, _i]),
+    "cpg_qwen3_paged_free_pages": (_i, [_vp]),
+    "cpg_qwen3_paged_logits": (_vp, [_vp, ctypes.POINTER(_i)]),
     "cpg_ctx_x": (_vp, [_vp]),
     "cpg_ctx_topk": (_vp, [_vp]),
     "cpg_ctx_profile": (_i, [_vp, _i]),

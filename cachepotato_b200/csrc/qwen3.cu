@@ -23,7 +23,7 @@
 #include <math.h>
 
 #include <algorithm>
-
+#include <new>
 #include <vector>
 
 #include "common.cuh"
@@ -804,6 +804,32 @@ __global__ void k_batch_advance(const int *__restrict__ next, int *__restrict__ 
     if (threadIdx.x == 0) *d_step = step + 1;
 }
 
+// Rows row[i] of x (., D), one block each: a mixed step's last row per sequence, for the head.
+__global__ void __launch_bounds__(256) k_pick_rows(const float *__restrict__ x, const int *__restrict__ row, int D,
+                                                    float *__restrict__ out) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const float *src = x + (size_t)row[blockIdx.x] * D;
+    for (int k = threadIdx.x; k < D; k += blockDim.x) out[(size_t)blockIdx.x * D + k] = src[k];
+}
+
+// After a step of single tokens over the paged cache: every sequence advances by one position, its
+// argmax becomes its next input id and is recorded at out[step·n + t], step = *d_step, which advances.
+__global__ void k_paged_advance(const int *__restrict__ next, int *__restrict__ ids, int *__restrict__ pos0, int n,
+                                int *__restrict__ out, int *__restrict__ d_step) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int step = *d_step;
+    __syncthreads();
+    for (int t = threadIdx.x; t < n; t += blockDim.x) {
+        const int id = next[t];
+        pos0[t] += 1;
+        ids[t] = id;
+        out[(size_t)step * n + t] = id;
+    }
+    if (threadIdx.x == 0) *d_step = step + 1;
+}
+
 int matvec_launch(float *out, const float *x, cpg_tensor w, int n_in, int n_out, int T, cudaStream_t s);
 struct GemvSeg {
     const uint8_t *w;
@@ -1066,6 +1092,17 @@ extern "C" void cpg_qwen3_destroy(cpg_qwen3 *m) {
 // token t is the new token of slot tok_slot[t] at position tok_pos[t] (a step of several
 // sequences). The head runs on the last row (one sequence) or on every row (several), into
 // logits (rows, V) and the argmax into d_next[row].
+// With `pg` set the rows are a mixed step over the paged cache instead: pg->batch says which rows
+// belong to which sequence, the head runs on the sequences' last rows (pg->last, or every row when
+// each sequence brings one).
+struct QwPaged {
+    cpg_kv *const *kv;              // one handle per layer
+    cpg_kv_batch batch;
+    const int *last;                // device: last row of each sequence; null: one row each
+    float *xlast;
+    void *ws;
+    size_t ws_bytes;
+};
 struct QwSeq {
     float *kv;
     int S, C;
@@ -1078,6 +1115,7 @@ struct QwSeq {
     float *logits, *am_v;
     int *am_i, *d_next;
     const QwDense *dn;              // several sequences: the dense.cu path, or null
+    const QwPaged *pg = nullptr;
 };
 
 // Enqueue T tokens (ids in m->d_ids[0..T)) through embed, the layers and the head. Nothing here
@@ -1135,15 +1173,25 @@ static int qwen3_enqueue(cpg_qwen3 *m, const QwSeq &sq, int T, cudaStream_t s) {
             if (!rc) rc = matvec_launch(m->vst, m->xn, A.wv, D, KD, T, s);
         }
         if (rc) return rc;
+        if (sq.pg) {
+            const QwPaged &pg = *sq.pg;
+            rc = cpg_kv_append(pg.kv[l], &pg.batch, CPG_T_F32, H, m->q, QD, m->kst, KD, m->vst, KD, A.q_norm, A.k_norm,
+                               m->eps, m->q, QD, s);
+            if (!rc) rc = cpg_kv_attend(pg.kv[l], &pg.batch, CPG_T_F32, H, m->q, QD, m->ao, QD,
+                                        1.0f / sqrtf((float)QW_HD), 0, pg.ws, pg.ws_bytes, s);
+            if (rc) return rc;
+        }
         const int warps = T * (H + KV);
         AttnNorm nr{};                               // new tokens, one per sequence: fused into the attention
-        if (T == 1 || multi) nr = AttnNorm{m->kst, m->vst, A.q_norm, A.k_norm, m->theta, m->eps, 1};
+        if (sq.pg) {
+        } else if (T == 1 || multi) nr = AttnNorm{m->kst, m->vst, A.q_norm, A.k_norm, m->theta, m->eps, 1};
         else
             CPG_CUDA(launch_pdl(k_qk_norm_rope, dim3((warps + 7) / 8), dim3(256), 0, s, m->q, (const float *)m->kst,
                                 (const float *)m->vst, kc, vc, T, sq.d_pos, H, KV, A.q_norm, A.k_norm,
                                 m->theta, m->eps));
         const int n_cap = sq.n_cap;                                  // prompt: positions known here
-        if (!multi && T >= QW_DENSE_MIN_T && attention_prompt_smem(n_cap) <= m->ap_smem) {
+        if (sq.pg) {
+        } else if (!multi && T >= QW_DENSE_MIN_T && attention_prompt_smem(n_cap) <= m->ap_smem) {
             k_attention_prompt<<<dim3(H, (T + AP_QT - 1) / AP_QT), 256, attention_prompt_smem(n_cap), s>>>(
                 (const float *)m->q, (const float *)kc, (const float *)vc, sq.d_pos, T, H, KV, n_cap, m->ao);
             CPG_CUDA(cudaGetLastError());
@@ -1181,11 +1229,15 @@ static int qwen3_enqueue(cpg_qwen3 *m, const QwSeq &sq, int T, cudaStream_t s) {
     }
     // head: RMSNorm with final_norm fused into the lm_head GEMV, of the last position (one
     // sequence) or of every row (one new token per sequence)
-    const int hr = multi ? T : 1;
+    const int hr = sq.pg ? sq.pg->batch.n_seqs : multi ? T : 1;
     const float *xl = m->x + (size_t)(T - hr) * D;
+    if (sq.pg && sq.pg->last) {
+        CPG_CUDA(launch_pdl(k_pick_rows, dim3(hr), dim3(256), 0, s, (const float *)m->x, sq.pg->last, D, sq.pg->xlast));
+        xl = sq.pg->xlast;
+    }
     const GemvSeg hseg{(const uint8_t *)m->lm_head.p, sq.logits, m->V};
     int rc = 1;
-    if (multi && sq.dn && sq.dn->head && hr >= QW_DENSE_DEC_MIN_T && hr <= QW_DENSE_DEC_MAX_T) {
+    if ((multi || sq.pg) && sq.dn && sq.dn->head && hr >= QW_DENSE_DEC_MIN_T && hr <= QW_DENSE_DEC_MAX_T) {
         const uint8_t *tl[1] = {sq.dn->head};
         const int rows[1] = {m->V};
         float *const outs[1] = {sq.logits};
@@ -1537,4 +1589,286 @@ extern "C" int cpg_qwen3_batch_position(const cpg_qwen3_batch *b, int slot) {
 extern "C" const float *cpg_qwen3_batch_logits(const cpg_qwen3_batch *b, int *rows) {
     if (rows) *rows = b ? b->last_rows : 0;
     return b ? b->logits : nullptr;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many sequences over a pool of pages (cpg_kv_append / cpg_kv_attend in every layer): a step takes
+// chunks of prompts and single tokens together, and memory follows what the sequences hold instead of
+// n_slots times max_ctx. The reference has one contiguous cache (qwen3_moe.h:40-70); per sequence the
+// arithmetic is that of the model's own path, the angles of its rotation included.
+struct cpg_qwen3_paged {
+    cpg_qwen3 *m = nullptr;
+    int S = 0, C = 0, P = 0, W = 0, n_pages = 0;         // slots, positions each, page size, table width, pages
+    uint8_t *pool = nullptr;                             // L x 2 x n_pages x P x KV x hd
+    std::vector<cpg_kv *> kv;                            // a handle per layer, one status word
+    std::vector<int> free_pages, pos;                    // pos: -1 = empty slot
+    std::vector<std::vector<int>> held;                  // a slot's pages, in order
+    int *d_step_in = nullptr, *h_step_in = nullptr;      // q_start (S + 1), pos0 (S), last (S), tables (S x W)
+    int *d_next = nullptr, *d_step = nullptr, *d_out = nullptr, *h_out = nullptr;
+    float *logits = nullptr, *am_v = nullptr, *xlast = nullptr;
+    int *am_i = nullptr;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    int last_rows = 0;
+    std::vector<cudaGraphExec_t> graphs;                 // a step of n single tokens, by n
+};
+
+namespace cpg {
+int kv_create_like(const cpg_kv_desc *d, const cpg_kv *like, cpg_kv **out);
+}  // namespace cpg
+
+static void paged_free(cpg_qwen3_paged *p) {
+    for (cudaGraphExec_t g : p->graphs)
+        if (g) cudaGraphExecDestroy(g);
+    for (size_t l = p->kv.size(); l > 0; --l) cpg_kv_destroy(p->kv[l - 1]);
+    cudaFree(p->pool); cudaFree(p->d_step_in); cudaFree(p->d_next); cudaFree(p->d_step); cudaFree(p->d_out);
+    cudaFree(p->logits); cudaFree(p->am_v); cudaFree(p->am_i); cudaFree(p->xlast); cudaFree(p->ws);
+    if (p->h_step_in) cudaFreeHost(p->h_step_in);
+    if (p->h_out) cudaFreeHost(p->h_out);
+    delete p;
+}
+
+extern "C" int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, int page_size, int n_pages, int type,
+                                      cpg_qwen3_paged **out) {
+    const char *fn = "cpg_qwen3_paged_create";
+    CPG_REQUIRE(m && out, "%s: null argument", fn);
+    *out = nullptr;
+    CPG_REQUIRE(n_slots >= 1 && n_slots <= m->max_ctx, "%s: n_slots %d (1..the model's max_ctx %d)", fn, n_slots, m->max_ctx);
+    CPG_REQUIRE(max_ctx >= 1 && max_ctx <= (1 << 30), "%s: max_ctx %d", fn, max_ctx);
+    CPG_REQUIRE(page_size >= 8 && page_size % 8 == 0 && page_size <= 65536, "%s: page_size %d (a multiple of 8, at most 65536)", fn, page_size);
+    CPG_REQUIRE(n_pages >= 1, "%s: n_pages %d", fn, n_pages);
+    CPG_REQUIRE(type == CPG_T_F32 || type == CPG_T_F16 || type == CPG_T_BF16, "%s: element type %d", fn, type);
+    cpg_qwen3_paged *p = new (std::nothrow) cpg_qwen3_paged();
+    if (!p) {
+        set_error("%s: host allocation failed", fn);
+        return CPG_ENOMEM;
+    }
+    p->m = m;
+    p->S = n_slots; p->C = max_ctx; p->P = page_size; p->n_pages = n_pages;
+    p->W = (max_ctx + page_size - 1) / page_size;
+    p->pos.assign(n_slots, -1);
+    p->held.resize(n_slots);
+    p->graphs.assign(n_slots + 1, nullptr);
+    for (int i = n_pages - 1; i >= 0; --i) p->free_pages.push_back(i);
+    const size_t S = n_slots, es = type == CPG_T_F32 ? 4 : 2, KD = (size_t)m->KV * QW_HD;
+    const size_t one = (size_t)n_pages * page_size * KD * es;
+    const size_t in_ints = 3 * S + 1 + S * p->W;
+    cudaError_t ce = cudaMalloc(&p->pool, (size_t)m->L * 2 * one);
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->d_step_in, in_ints * sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMallocHost(&p->h_step_in, (in_ints + m->max_ctx) * sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->d_next, S * sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->d_step, sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->d_out, S * sizeof(int) * (size_t)m->max_ctx);
+    if (ce == cudaSuccess) ce = cudaMallocHost(&p->h_out, (S + 1) * sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->logits, S * (size_t)m->V * sizeof(float));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->am_v, S * AM_BLOCKS * sizeof(float));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->am_i, S * AM_BLOCKS * sizeof(int));
+    if (ce == cudaSuccess) ce = cudaMalloc(&p->xlast, S * (size_t)m->D * sizeof(float));
+    int rc = ce == cudaSuccess ? CPG_OK : cuda_fail(ce, fn);
+    for (int l = 0; l < m->L && !rc; ++l) {
+        uint8_t *k = p->pool + (size_t)(2 * l) * one;
+        const cpg_kv_desc d{m->KV, QW_HD, page_size, n_pages, type, k, k + one, (long)(page_size * KD), (long)KD, QW_HD,
+                            QW_HD, m->theta, 1};
+        cpg_kv *h = nullptr;
+        rc = kv_create_like(&d, l ? p->kv[0] : nullptr, &h);
+        if (!rc) p->kv.push_back(h);
+    }
+    if (!rc) {
+        p->ws_bytes = cpg_kv_attend_workspace_bytes(p->kv[0], m->H);
+        ce = cudaMalloc(&p->ws, p->ws_bytes);
+        if (ce == cudaSuccess) ce = cudaMemsetAsync(p->ws, 0, p->ws_bytes, m->s);
+        if (ce == cudaSuccess) ce = cudaStreamSynchronize(m->s);
+        if (ce != cudaSuccess) rc = cuda_fail(ce, fn);
+    }
+    if (!rc && n_slots >= QW_DENSE_DEC_MIN_T && m->dn.attn.empty()) rc = build_dense(m);
+    if (rc) {
+        paged_free(p);
+        return rc;
+    }
+    *out = p;
+    return CPG_OK;
+}
+
+extern "C" void cpg_qwen3_paged_destroy(cpg_qwen3_paged *p) {
+    if (!p) return;
+    cudaStreamSynchronize(p->m->s);
+    paged_free(p);
+}
+
+// The named slots: distinct, each with room for its new rows; pages for all of them, or none taken.
+static int paged_reserve(cpg_qwen3_paged *p, const int *slots, const int *n_new, int n, int every, const char *fn) {
+    CPG_REQUIRE(slots && n >= 1 && n <= p->S, "%s: %d sequences (1..%d)", fn, n, p->S);
+    std::vector<char> seen(p->S, 0);
+    long need = 0;
+    for (int i = 0; i < n; ++i) {
+        const int j = slots[i], c = n_new ? n_new[i] : every;
+        CPG_REQUIRE(j >= 0 && j < p->S, "%s: slot %d of %d", fn, j, p->S);
+        CPG_REQUIRE(!seen[j], "%s: slot %d named twice", fn, j);
+        seen[j] = 1;
+        CPG_REQUIRE(c >= 1, "%s: slot %d takes %d tokens", fn, j, c);
+        CPG_REQUIRE(n_new || p->pos[j] >= 1, "%s: slot %d holds no sequence", fn, j);
+        const long to = (long)std::max(p->pos[j], 0) + c;
+        CPG_REQUIRE(to <= p->C, "%s: slot %d at position %d: %d more tokens pass max_ctx %d", fn, j, std::max(p->pos[j], 0), c, p->C);
+        need += std::max(0l, (to + p->P - 1) / p->P - (long)p->held[j].size());
+    }
+    if (need > (long)p->free_pages.size()) {
+        set_error("%s: the step needs %ld more pages, the pool has %zu free", fn, need, p->free_pages.size());
+        return CPG_ENOMEM;
+    }
+    for (int i = 0; i < n; ++i) {
+        const int j = slots[i];
+        const int pages = (std::max(p->pos[j], 0) + (n_new ? n_new[i] : every) + p->P - 1) / p->P;
+        while ((int)p->held[j].size() < pages) {
+            p->held[j].push_back(p->free_pages.back());
+            p->free_pages.pop_back();
+        }
+    }
+    return CPG_OK;
+}
+
+// The step's arrays and ids to the device; returns the rows' description.
+static int paged_upload(cpg_qwen3_paged *p, const int *slots, const int *n_new, const int *ids, int n, int T, QwPaged *pg) {
+    cpg_qwen3 *m = p->m;
+    const int S = p->S, W = p->W;
+    int *h = p->h_step_in, *start = h, *pos0 = h + S + 1, *last = pos0 + S, *table = last + S, *h_ids = table + (size_t)S * W;
+    int at = 0, most = 0;
+    for (int i = 0; i < n; ++i) {
+        const int c = n_new ? n_new[i] : 1;
+        start[i] = at;
+        pos0[i] = std::max(p->pos[slots[i]], 0);
+        last[i] = at + c - 1;
+        at += c;
+        most = std::max(most, c);
+        const std::vector<int> &held = p->held[slots[i]];
+        std::copy(held.begin(), held.end(), table + (size_t)i * W);
+    }
+    start[n] = at;
+    std::copy(ids, ids + T, h_ids);
+    const size_t ints = 3 * (size_t)S + 1 + (size_t)n * W;
+    CPG_CUDA(cudaMemcpyAsync(p->d_step_in, h, ints * sizeof(int), cudaMemcpyHostToDevice, m->s));
+    CPG_CUDA(cudaMemcpyAsync(m->d_ids, h_ids, sizeof(int) * (size_t)T, cudaMemcpyHostToDevice, m->s));
+    int *d = p->d_step_in;
+    *pg = QwPaged{p->kv.data(), cpg_kv_batch{n, T, d, d + S + 1, d + 3 * S + 1, W, W, most}, most > 1 ? d + 2 * S + 1 : nullptr,
+                  p->xlast, p->ws, p->ws_bytes};
+    return CPG_OK;
+}
+
+static QwSeq paged_seq(cpg_qwen3_paged *p, const QwPaged *pg) {
+    QwSeq sq{};
+    sq.S = 1;
+    sq.C = p->C;
+    sq.slot = 0;
+    sq.logits = p->logits;
+    sq.am_v = p->am_v;
+    sq.am_i = p->am_i;
+    sq.d_next = p->d_next;
+    sq.dn = p->m->dn.attn.empty() ? nullptr : &p->m->dn;
+    sq.pg = pg;
+    return sq;
+}
+
+// n single tokens, n_steps times, each feeding the previous argmax: the step captured once per n.
+static int paged_run(cpg_qwen3_paged *p, const QwPaged &pg, int n, int n_steps) {
+    cpg_qwen3 *m = p->m;
+    CPG_CUDA(cudaMemsetAsync(p->d_step, 0, sizeof(int), m->s));
+    if (!p->graphs[n]) {
+        const QwSeq sq = paged_seq(p, &pg);
+        cudaGraph_t g = nullptr;
+        CPG_CUDA(cudaStreamBeginCapture(m->s, cudaStreamCaptureModeThreadLocal));
+        int rc = qwen3_enqueue(m, sq, n, m->s);
+        if (!rc) {
+            k_paged_advance<<<1, 256, 0, m->s>>>(p->d_next, m->d_ids, const_cast<int *>(pg.batch.pos0), n, p->d_out, p->d_step);
+            const cudaError_t le = cudaGetLastError();
+            if (le != cudaSuccess) rc = cuda_fail(le, "cpg_qwen3_paged: step launch");
+        }
+        const cudaError_t ce = cudaStreamEndCapture(m->s, &g);
+        if (rc) {
+            if (g) cudaGraphDestroy(g);
+            return rc;
+        }
+        if (ce != cudaSuccess) return cuda_fail(ce, "cpg_qwen3_paged: step capture");
+        const cudaError_t ie = cudaGraphInstantiate(&p->graphs[n], g, 0);
+        cudaGraphDestroy(g);
+        if (ie != cudaSuccess) return cuda_fail(ie, "cpg_qwen3_paged: step instantiate");
+    }
+    for (int i = 0; i < n_steps; ++i) CPG_CUDA(cudaGraphLaunch(p->graphs[n], m->s));
+    return CPG_OK;
+}
+
+static int paged_status(cpg_qwen3_paged *p, const char *fn) {
+    const int rc = cpg_kv_check(p->kv[0], p->m->s);
+    return rc ? rc : qwen3_status(p->m, fn);
+}
+
+extern "C" int cpg_qwen3_paged_step(cpg_qwen3_paged *p, const int *slots, const int *n_new, const int *ids, int n,
+                                    int *next_ids) {
+    const char *fn = "cpg_qwen3_paged_step";
+    CPG_REQUIRE(p && slots && n_new && ids && next_ids, "%s: null argument", fn);
+    cpg_qwen3 *m = p->m;
+    CPG_REQUIRE(n >= 1 && n <= p->S, "%s: %d sequences (1..%d)", fn, n, p->S);
+    long T = 0;
+    for (int i = 0; i < n; ++i) {
+        CPG_REQUIRE(n_new[i] >= 1 && n_new[i] <= m->max_ctx, "%s: sequence %d takes %d tokens", fn, i, n_new[i]);
+        T += n_new[i];
+    }
+    CPG_REQUIRE(T <= m->max_ctx, "%s: %ld tokens in a step (at most the model's max_ctx %d)", fn, T, m->max_ctx);
+    for (long t = 0; t < T; ++t) CPG_REQUIRE(ids[t] >= 0 && ids[t] < m->V, "%s: id %d out of range", fn, ids[t]);
+    int rc = paged_reserve(p, slots, n_new, n, 0, fn);
+    if (rc) return rc;
+    QwPaged pg;
+    rc = paged_upload(p, slots, n_new, ids, n, (int)T, &pg);
+    if (rc) return rc;
+    if (T == n) {
+        rc = paged_run(p, pg, n, 1);
+    } else {
+        rc = qwen3_enqueue(m, paged_seq(p, &pg), (int)T, m->s);
+    }
+    if (rc) return rc;
+    CPG_CUDA(cudaMemcpyAsync(p->h_out, p->d_next, sizeof(int) * n, cudaMemcpyDeviceToHost, m->s));
+    CPG_CUDA(cudaStreamSynchronize(m->s));
+    for (int i = 0; i < n; ++i) {
+        p->pos[slots[i]] = std::max(p->pos[slots[i]], 0) + n_new[i];
+        next_ids[i] = p->h_out[i];
+    }
+    p->last_rows = n;
+    return paged_status(p, fn);
+}
+
+extern "C" int cpg_qwen3_paged_generate(cpg_qwen3_paged *p, const int *slots, const int *ids, int n, int n_steps, int *out_ids) {
+    const char *fn = "cpg_qwen3_paged_generate";
+    CPG_REQUIRE(p && slots && ids && out_ids, "%s: null argument", fn);
+    cpg_qwen3 *m = p->m;
+    CPG_REQUIRE(n_steps >= 1 && n_steps <= m->max_ctx, "%s: %d steps (1..the model's max_ctx %d)", fn, n_steps, m->max_ctx);
+    CPG_REQUIRE(n >= 1 && n <= p->S, "%s: %d sequences (1..%d)", fn, n, p->S);
+    for (int t = 0; t < n; ++t) CPG_REQUIRE(ids[t] >= 0 && ids[t] < m->V, "%s: id %d out of range", fn, ids[t]);
+    int rc = paged_reserve(p, slots, nullptr, n, n_steps, fn);
+    if (rc) return rc;
+    QwPaged pg;
+    rc = paged_upload(p, slots, nullptr, ids, n, n, &pg);
+    if (!rc) rc = paged_run(p, pg, n, n_steps);
+    if (rc) return rc;
+    CPG_CUDA(cudaMemcpyAsync(out_ids, p->d_out, sizeof(int) * (size_t)n * n_steps, cudaMemcpyDeviceToHost, m->s));
+    CPG_CUDA(cudaStreamSynchronize(m->s));
+    for (int i = 0; i < n; ++i) p->pos[slots[i]] += n_steps;
+    p->last_rows = n;
+    return paged_status(p, fn);
+}
+
+extern "C" int cpg_qwen3_paged_drop(cpg_qwen3_paged *p, int slot) {
+    CPG_REQUIRE(p && slot >= 0 && slot < p->S, "cpg_qwen3_paged_drop: slot %d", slot);
+    std::vector<int> &held = p->held[slot];
+    p->free_pages.insert(p->free_pages.end(), held.rbegin(), held.rend());
+    held.clear();
+    p->pos[slot] = -1;
+    return CPG_OK;
+}
+
+extern "C" int cpg_qwen3_paged_position(const cpg_qwen3_paged *p, int slot) {
+    return p && slot >= 0 && slot < p->S ? p->pos[slot] : -1;
+}
+extern "C" int cpg_qwen3_paged_free_pages(const cpg_qwen3_paged *p) { return p ? (int)p->free_pages.size() : 0; }
+
+extern "C" const float *cpg_qwen3_paged_logits(const cpg_qwen3_paged *p, int *rows) {
+    if (rows) *rows = p ? p->last_rows : 0;
+    return p ? p->logits : nullptr;
 }

@@ -493,6 +493,70 @@ class Qwen3Batch:
             pass
 
 
+class Qwen3Paged:
+    """cpg_qwen3_paged: many sequences over a pool of pages. step(slots, chunks) takes the next chunk
+    of each named slot's prompt, or its next token, together; drop(slot) ends a sequence. cache: "f32"
+    (the ids of Qwen3Model.generate), "f16" or "bf16"."""
+
+    def __init__(self, model: Qwen3Model, n_slots: int, max_ctx: int, *, n_pages: int, page_size: int = 64, cache: str = "f32"):
+        types = {"f32": _lib.T_F32, "f16": _lib.T_F16, "bf16": _lib.T_BF16}
+        if cache not in types:
+            raise _lib.CpgError(_lib.CPG_EINVAL, f"cache {cache!r}: one of {sorted(types)}")
+        h = ctypes.c_void_p()
+        check(lib().cpg_qwen3_paged_create(model.handle, n_slots, max_ctx, page_size, n_pages, types[cache], ctypes.byref(h)))
+        self.handle, self.model, self.vocab, self.n_slots = h, model, model.vocab, n_slots
+
+    def step(self, slots, chunks) -> np.ndarray:
+        """chunks[i]: the new ids of slots[i]. The argmax after each slot's last id."""
+        slots = np.ascontiguousarray(slots, dtype=np.int32)
+        chunks = [np.atleast_1d(np.asarray(c, dtype=np.int32)) for c in chunks]
+        assert len(slots) == len(chunks)
+        counts = np.array([len(c) for c in chunks], np.int32)
+        ids = np.concatenate(chunks) if chunks else np.zeros(0, np.int32)
+        out = np.zeros(len(slots), np.int32)
+        check(lib().cpg_qwen3_paged_step(self.handle, slots.ctypes.data, counts.ctypes.data, ids.ctypes.data, len(slots),
+                                         out.ctypes.data))
+        return out
+
+    def generate(self, slots, ids, n_steps: int) -> np.ndarray:
+        """(n_steps, len(slots)) ids: row s = the ids step s produced."""
+        slots = np.ascontiguousarray(slots, dtype=np.int32)
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        assert len(slots) == len(ids)
+        out = np.zeros((max(n_steps, 0), len(slots)), np.int32)
+        check(lib().cpg_qwen3_paged_generate(self.handle, slots.ctypes.data, ids.ctypes.data, len(slots), n_steps,
+                                             out.ctypes.data))
+        return out
+
+    def drop(self, slot: int) -> None:
+        check(lib().cpg_qwen3_paged_drop(self.handle, int(slot)))
+
+    def position(self, slot: int) -> int:
+        return int(lib().cpg_qwen3_paged_position(self.handle, int(slot)))
+
+    def free_pages(self) -> int:
+        return int(lib().cpg_qwen3_paged_free_pages(self.handle))
+
+    def logits(self):
+        """The last call's logits as a (rows, vocab) device tensor (a view; valid until the next call)."""
+        torch = _torch()
+        from .workload import device_view
+        rows = ctypes.c_int()
+        p = int(lib().cpg_qwen3_paged_logits(self.handle, ctypes.byref(rows)))
+        return device_view(torch, p, rows.value * self.vocab * 4, "f4").view(rows.value, self.vocab)
+
+    def close(self) -> None:
+        if self.handle is not None and self.handle.value:
+            lib().cpg_qwen3_paged_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class DecodeContext:
     """cpg_ctx: the host-buffer decode loop (run_layers' MoE half, cachepotato.c:149-166)."""
 

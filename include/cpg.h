@@ -371,6 +371,31 @@ int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads
  * the pools and the rows was touched), CPG_ETIMEOUT if a bounded device wait gave up. */
 int cpg_kv_check(const cpg_kv *kv, void *stream);
 
+/* ------------------------------------------- many sequences over a pool of pages
+ * Like a batch, but the sequences share n_pages pages per layer (append and attention above, f32,
+ * f16 or bf16 elements) and a step takes chunks of prompts and single tokens together. A sequence
+ * holds pages for the positions it has, so n_slots times max_ctx may be far more than the pool; a step
+ * that needs more pages than are free is refused with CPG_ENOMEM and changes nothing. With an f32
+ * cache the ids per sequence are those of cpg_qwen3_generate; a 16-bit one rounds keys and values.
+ * Runs on the model's stream and scratch: not at the same time as its own sequence or a batch. */
+typedef struct cpg_qwen3_paged cpg_qwen3_paged;
+int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, int page_size, int n_pages, int type,
+                           cpg_qwen3_paged **out);
+void cpg_qwen3_paged_destroy(cpg_qwen3_paged *p);
+/* One step: slots[i] (distinct) takes n_new[i] >= 1 ids, ids being theirs one after another (at most
+   the model's max_ctx in all): the next chunk of its prompt or its next token; an empty slot starts a
+   sequence at position 0. next_ids[i] = argmax after its last one. */
+int cpg_qwen3_paged_step(cpg_qwen3_paged *p, const int *slots, const int *n_new, const int *ids, int n,
+                         int *next_ids);
+/* n_steps single tokens for each named slot, each feeding the previous argmax; out_ids (n_steps, n). */
+int cpg_qwen3_paged_generate(cpg_qwen3_paged *p, const int *slots, const int *ids, int n, int n_steps,
+                             int *out_ids);
+int cpg_qwen3_paged_drop(cpg_qwen3_paged *p, int slot);          /* ends its sequence, frees its pages */
+int cpg_qwen3_paged_position(const cpg_qwen3_paged *p, int slot); /* -1: empty slot */
+int cpg_qwen3_paged_free_pages(const cpg_qwen3_paged *p);
+/* Device logits of the last call, *rows rows of vocab f32 in its slot order. */
+const float *cpg_qwen3_paged_logits(const cpg_qwen3_paged *p, int *rows);
+
 /* ============================================================== decode loop (host buffers)
  * A context owns a stream, a workspace and device activation buffers on one device. */
 typedef struct cpg_ctx cpg_ctx;
