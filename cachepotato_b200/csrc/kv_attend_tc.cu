@@ -19,6 +19,8 @@
 //           warp 8          producer: q tiles and the ring of K and V tiles, tensor TMA
 //           warp 9          tcgen05.mma: S = q·K^T (both operands in shared memory), O += P·V (P from
 //                           TMEM). While one row tile is in its softmax the other's products run.
+//           warp 10         clears the places of an item's last V tile that lie in its last page behind
+//                           the last position (they may hold anything, and 0 · NaN is NaN)
 //           TMEM: S0 S1 | O0 O1, 128 columns each; P lies over its S.
 //   order   The tensor core runs what one thread issues in order, so q·k of the next tile may be
 //           issued behind the p·v that still reads P from the same columns, and a finished q·k says
@@ -28,13 +30,15 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv_attend.cuh"
 
 namespace cpg {
 
 constexpr int KT_TILE = 128, KT_ROWS = 128;               // positions and rows of an MMA tile
-constexpr int KT_THREADS = 384, KT_PRODUCER = 8, KT_MMA = 9;
+constexpr int KT_THREADS = 384, KT_PRODUCER = 8, KT_MMA = 9, KT_FIXER = 10;
+constexpr int KT_POLY = 0;                                // pairs in 8 whose exponentials are polynomials
 constexpr int KT_FIXED = 2;                               // units an item's begin and end are worth (see KD_FIXED)
 template <int HD> constexpr int kt_unit() { return KT_TILE * HD * 2; }
 template <int HD> constexpr int kt_units() { return HD == 128 ? 5 : 8; }
@@ -134,6 +138,7 @@ struct KtRows {
 };
 
 __device__ __forceinline__ bool kt_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
+    if (mbar_try_wait(smem_u32(bar), parity)) return true;
     if (*abort_flag) return false;
     if (mbar_wait(bar, parity)) return true;
     *abort_flag = 1;
@@ -144,6 +149,56 @@ __device__ __forceinline__ bool kt_wait(uint64_t *bar, uint32_t parity, volatile
 // The same for a whole warp, which goes on or leaves together.
 __device__ __forceinline__ bool kt_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
     return __all_sync(0xffffffffu, kt_wait(bar, parity, abort_flag, status));
+}
+
+// Whether a V tile with `end` places up to the item's last position has more in that one's box.
+__device__ __forceinline__ bool kt_fix(const AttendArgs &a, int end) { return end < KT_TILE && end % a.box; }
+
+// Two f32 in one 64-bit register, worked on by one instruction (sm_100).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two numbers on the multiply-add pipe: n = round(x) by adding 1.5 · 2^23, a polynomial of
+// least largest relative error for 2^(x - n) on [-1/2, 1/2] (Remez exchange: 2^-13.7 with degree 3,
+// 2^-18.6 with degree 4, against 2^-9 and 2^-12 of the rounding that follows), n added to the
+// exponent. For x < 128; below 2^-125 it gives 2^-125.
+template <int DEG>
+__device__ __forceinline__ f32x2 ex2_poly2(f32x2 x) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+    const f32x2 t = add2(x, pack2(12582912.0f, 12582912.0f));
+    const f32x2 r = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
+    f32x2 p;
+    if (DEG == 3) {
+        p = fma2(r, pack2(0.05517167f, 0.05517167f), pack2(0.24261113f, 0.24261113f));
+        p = fma2(r, p, pack2(0.69326097f, 0.69326097f));
+        p = fma2(r, p, pack2(0.99992806f, 0.99992806f));
+    } else {
+        p = fma2(r, pack2(0.0095701021f, 0.0095701021f), pack2(0.055917859f, 0.055917859f));
+        p = fma2(r, p, pack2(0.24024744f, 0.24024744f));
+        p = fma2(r, p, pack2(0.69312179f, 0.69312179f));
+        p = fma2(r, p, pack2(0.99999928f, 0.99999928f));
+    }
+    float p0, p1, t0, t1;
+    unpack2(p, p0, p1);
+    unpack2(t, t0, t1);
+    return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
+                 __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
 }
 
 // Nothing that uses r may be moved before this point (the wait for the loads that fill it).
@@ -167,17 +222,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     constexpr uint32_t ID_QK = umma_idesc_f16(128, KT_TILE) | FMT, ID_PV = umma_idesc_f16(128, HD) | FMT | UMMA_B_MN;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain;
+    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, asked[NU], fixed[NU], s_full[2], p_full[2], o_full[2], drain;
     __shared__ long s_scan[KT_THREADS / 32], s_cut[2];
     __shared__ KtCursor s_cur;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_last[2];
+    __shared__ int s_abort, s_last[2], s_ask[NU][3];     // a V tile to clear: ring slot, its fill's parity, first place
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = a.H / a.c.KV, TT = KT_ROWS / G, Q = 2 * TT;             // tokens of a row tile, of a pair
     if (tid == 0) {
         for (int i = 0; i < NU; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
+            mbar_init(&asked[i], 1);
+            mbar_init(&fixed[i], 1);
         }
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
@@ -295,7 +352,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
         if (warp == KT_PRODUCER) {
             // ---------------- producer: lane b loads box b of every unit
             const int groups = KT_TILE / a.box, boxes = groups * PARTS;
-            int slot = 0, turn = 0, items = 0;
+            int slot = 0, turn = 0, items = 0, asks = 0;
             bool ok = true;
             for (long u = u0; u < u1 && ok;) {
                 if (!begin(u)) break;
@@ -331,6 +388,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         if (lane < boxes)
                             tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
                                         lane % PARTS * 64, place, cur.kh, page, &full[slot]);
+                        if (half && kt_fix(a, cur.hi - j0)) {
+                            if (lane == 0) {
+                                s_ask[asks % NU][0] = slot;
+                                s_ask[asks % NU][1] = turn & 1;
+                                s_ask[asks % NU][2] = cur.hi - j0;
+                                mbar_arrive(&asked[asks % NU]);
+                            }
+                            ++asks;
+                        }
                         if (++slot == NU) {
                             slot = 0;
                             ++turn;
@@ -349,107 +415,122 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                 if (items) mbar_wait(&q_full, (uint32_t)(items - 1) & 1u);
             }
         } else if (warp == KT_MMA) {
-            // ---------------- tensor core (lane 0 issues)
-            int ks = 0, vs = 1;                           // ring slots of the next K and V
-            uint32_t kp = 0, vp = 0, pp[2] = {0, 0}, qp = 0;
-            auto step2 = [&](int &s, uint32_t &ph) {
-                s += 2;
-                if (s >= NU) {
-                    s -= NU;
-                    ph ^= 1;
-                }
-            };
-            bool ok = true;
-            for (long u = u0; u < u1 && ok;) {
-                if (!begin(u)) break;
-                const KtRows rows[2] = {KtRows(a, cur, Q, 0), KtRows(a, cur, Q, 1)};
-                const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                const int first = (cur.lo_t + cur.kt) * KT_TILE;
-                if (!kt_wait_warp(&q_full, qp, abort_flag, status)) break;
-                qp ^= 1;
-                bool begun[2] = {false, false};
-                auto qk = [&](int x, int i) {             // S_x = q_x · K_i^T
-                    if (lane == 0) {
-#pragma unroll
-                        for (int k = 0; k < HD / 16; ++k)
-                            umma_f16(tmem + x * 128, umma_desc_sw128(sq + x * QT + k / 4 * COL + k % 4 * 32),
-                                     umma_desc_sw128(ring + ks * UNIT + k / 4 * COL + k % 4 * 32), ID_QK, k ? 1u : 0u);
-                        umma_commit(&s_full[x]);
+            // ---------------- tensor core: one elected lane waits and issues
+            if (elect_one()) {
+                int ks = 0, vs = 1;                       // ring slots of the next K and V
+                uint32_t kp = 0, vp = 0, pp0 = 0, pp1 = 0, qp = 0, fp = 0;               // fp: a bit per slot
+                auto step2 = [&](int &s, uint32_t &ph) {
+                    s += 2;
+                    if (s >= NU) {
+                        s -= NU;
+                        ph ^= 1;
                     }
                 };
-                if (!kt_wait_warp(&full[ks], kp, abort_flag, status)) break;
-                tc_fence_after();
-                for (int x = 0; x < 2; ++x)
-                    if (rows[x].sees(first)) qk(x, 0);
-                if (lane == 0) {
+                auto wait = [&](uint64_t *bar, uint32_t parity) { return kt_wait(bar, parity, abort_flag, status); };
+                bool ok = true;
+                for (long u = u0; u < u1 && ok;) {
+                    if (!begin(u)) break;
+                    const KtRows r0(a, cur, Q, 0), r1(a, cur, Q, 1);
+                    const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
+                    const int first = (cur.lo_t + cur.kt) * KT_TILE;
+                    if (!wait(&q_full, qp)) break;
+                    qp ^= 1;
+                    bool begun0 = false, begun1 = false;
+                    // S_x = q_x · K^T from ring slot ks, O_x += P_x · V from slot vs; x = 0, 1
+                    auto qk = [&](int x) {
+                        const uint64_t dq = umma_desc_sw128(sq + x * QT), dk = umma_desc_sw128(ring + ks * UNIT);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint32_t at = (k / 4 * COL + k % 4 * 32) >> 4;       // of the descriptor's start
+                            umma_f16(tmem + x * 128, dq + at, dk + at, ID_QK, k ? 1u : 0u);
+                        }
+                        umma_commit(&s_full[x]);
+                    };
+                    auto pv = [&](int x, bool begun) {
+                        const uint64_t dv = umma_desc_sw128_mn(ring + vs * UNIT, COL);
+#pragma unroll
+                        for (int k = 0; k < KT_TILE / 16; ++k)
+                            umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, dv + (k * 2048 >> 4), ID_PV, begun || k ? 1u : 0u);
+                    };
+                    if (!wait(&full[ks], kp)) break;
+                    tc_fence_after();
+                    bool s0 = r0.sees(first), s1 = r1.sees(first);         // whether the row tiles see this unit
+                    if (s0) qk(0);
+                    if (s1) qk(1);
                     umma_commit(&empty[ks]);
                     if (n_here == 1) umma_commit(&q_empty);
-                }
-                step2(ks, kp);
-                for (int i = 0; i < n_here; ++i) {
-                    const int j0 = first + i * KT_TILE;
-                    if (!kt_wait_warp(&full[vs], vp, abort_flag, status)) {
-                        ok = false;
-                        break;
-                    }
-                    const int end = cur.hi - j0;          // places behind the last position may hold anything
-                    if (end < KT_TILE && end % a.box) {
-                        const int rows_z = (end + a.box - 1) / a.box * a.box - end;
-                        for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
-                            const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
-                            *reinterpret_cast<uint4 *>(smem + 2 * QT + vs * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+                    step2(ks, kp);
+                    for (int i = 0; i < n_here; ++i) {
+                        const int j0 = first + i * KT_TILE;
+                        const bool more = i + 1 < n_here;
+                        const bool n0 = more && r0.sees(j0 + KT_TILE), n1 = more && r1.sees(j0 + KT_TILE);
+                        ok = wait(&full[vs], vp) && (!more || wait(&full[ks], kp));
+                        if (ok && kt_fix(a, cur.hi - j0)) {
+                            ok = wait(&fixed[vs], fp >> vs & 1u);
+                            fp ^= 1u << vs;
                         }
-                        fence_async_smem();
-                        __syncwarp();
-                    }
-                    const bool more = i + 1 < n_here;
-                    bool have_k = false;
-                    for (int x = 0; x < 2; ++x) {
-                        if (rows[x].sees(j0)) {
-                            if (!kt_wait_warp(&p_full[x], pp[x], abort_flag, status)) {
-                                ok = false;
-                                break;
-                            }
-                            pp[x] ^= 1;
+                        if (!ok) break;
+                        if (s0) {
+                            ok = wait(&p_full[0], pp0);
+                            if (!ok) break;
+                            pp0 ^= 1;
                             tc_fence_after();
-                            if (lane == 0) {
-#pragma unroll
-                                for (int k = 0; k < KT_TILE / 16; ++k)
-                                    umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8,
-                                                umma_desc_sw128_mn(ring + vs * UNIT + k * 2048, COL), ID_PV, begun[x] || k ? 1u : 0u);
-                                if (!more || !rows[x].sees(j0 + KT_TILE)) umma_commit(&o_full[x]);
-                            }
-                            begun[x] = true;
+                            pv(0, begun0);
+                            begun0 = true;
+                            if (!n0) umma_commit(&o_full[0]);
                         }
-                        if (more && rows[x].sees(j0 + KT_TILE)) {
-                            if (!have_k) {
-                                if (!kt_wait_warp(&full[ks], kp, abort_flag, status)) {
-                                    ok = false;
-                                    break;
-                                }
-                                tc_fence_after();
-                                have_k = true;
-                            }
-                            qk(x, i + 1);
+                        if (n0) qk(0);
+                        if (s1) {
+                            ok = wait(&p_full[1], pp1);
+                            if (!ok) break;
+                            pp1 ^= 1;
+                            tc_fence_after();
+                            pv(1, begun1);
+                            begun1 = true;
+                            if (!n1) umma_commit(&o_full[1]);
                         }
+                        umma_commit(&empty[vs]);
+                        if (n1) qk(1);
+                        if (more) umma_commit(&empty[ks]);
+                        if (i + 2 == n_here) umma_commit(&q_empty);
+                        step2(vs, vp);
+                        if (more) step2(ks, kp);
+                        s0 = n0;
+                        s1 = n1;
                     }
-                    if (!ok) break;
-                    if (lane == 0) umma_commit(&empty[vs]);
-                    step2(vs, vp);
-                    if (more) {
-                        if (lane == 0) {
-                            umma_commit(&empty[ks]);
-                            if (i + 2 == n_here) umma_commit(&q_empty);
-                        }
-                        step2(ks, kp);
+                    u += n_here;
+                    if (u < u1) cur.next_item(a, Q);
+                }
+                // every MMA issued has finished before the block ends
+                umma_commit(&drain);
+                mbar_wait(&drain, 0);
+            }
+            __syncwarp();
+        } else if (warp == KT_FIXER) {
+            // the V tiles the producer asks for, in its order. A slot asked for is not filled again before
+            // it is cleared, so its barriers are never more than one phase from what is waited for.
+            int asks = 0;
+            for (long u = u0; u < u1;) {
+                if (!begin(u)) break;
+                const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
+                if (kt_fix(a, cur.hi - (cur.lo_t + cur.kt + n_here - 1) * KT_TILE)) {
+                    const int at = asks % NU;
+                    if (!kt_wait_warp(&asked[at], (uint32_t)(asks / NU) & 1u, abort_flag, status)) break;
+                    const int slot = s_ask[at][0], end = s_ask[at][2];
+                    if (!kt_wait_warp(&full[slot], (uint32_t)s_ask[at][1], abort_flag, status)) break;
+                    const int rows_z = (end + a.box - 1) / a.box * a.box - end;
+                    for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
+                        const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
+                        *reinterpret_cast<uint4 *>(smem + 2 * QT + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
                     }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&fixed[slot]);
+                    ++asks;
                 }
                 u += n_here;
                 if (u < u1) cur.next_item(a, Q);
             }
-            // every MMA issued has finished before the block ends
-            if (lane == 0) umma_commit(&drain);
-            mbar_wait(&drain, 0);
         }
     } else {
         // ---------------- softmax and output of row tile x, one thread per row
@@ -482,28 +563,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     for (int e = 0; e < 16; ++e)
                         if (c + e > top_j || c + e <= bottom_j) v[e] = 0xff800000u;
                 };
-                // weights of 16 scores -> 8 packed pairs; their sum added to `add`
-                auto weigh = [&](const uint32_t *v, float base, uint32_t *pk, float (&add)[4]) {
+                // weights of 16 scores -> 8 packed pairs; their sum added to `add`. POLY of the 8 pairs
+                // go to the multiply-add pipe
+                const f32x2 scale22 = pack2(a.scale2, a.scale2);
+                auto weigh = [&](const uint32_t *v, f32x2 minus, uint32_t *pk, f32x2 (&add)[2], auto poly) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float e0 = ex2(fmaf(__uint_as_float(v[2 * e]), a.scale2, -base));
-                        const float e1 = ex2(fmaf(__uint_as_float(v[2 * e + 1]), a.scale2, -base));
-                        add[e & 1] += e0;
-                        add[2 + (e & 1)] += e1;
+                        f32x2 x = fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale22, minus);
+                        float e0, e1;
+                        if ((e + 1) * decltype(poly)::value / 8 > e * decltype(poly)::value / 8) {
+                            x = ex2_poly2<HALF ? 4 : 3>(x);
+                            unpack2(x, e0, e1);
+                        } else {
+                            unpack2(x, e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            x = pack2(e0, e1);
+                        }
+                        add[e & 1] = add2(add[e & 1], x);
                         uint32_t w[1];
                         split_pair<HALF, 1>(e0, e1, w);
                         pk[e] = w[0];
                     }
                 };
+                using None = std::integral_constant<int, 0>;
+                using Some = std::integral_constant<int, KT_POLY>;
                 auto largest = [&](const uint32_t *v) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 2)
                         mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
                 };
-                float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                f32x2 add[2] = {0, 0};
                 uint32_t pk[64];                          // kept until m has proved large enough
-                if (begun) {
+                if (begun && !edge) {
                     const float base = m == -INFINITY ? 0.0f : m;
+                    const f32x2 minus = pack2(-base, -base);
                     uint32_t s[2][16];
                     tmem_ld16_nowait(tS, s[0]);
 #pragma unroll
@@ -512,9 +606,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         tmem_wait_ld();
                         settle16(v);
                         if (c < 7) tmem_ld16_nowait(tS + 16 * (c + 1), s[(c + 1) & 1]);
-                        if (edge) hide(v, 16 * c);
                         largest(v);
-                        weigh(v, base, pk + 8 * c, add);
+                        weigh(v, minus, pk + 8 * c, add, Some{});
                     }
                 } else {
 #pragma unroll 1
@@ -529,16 +622,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
                 const bool grow = top > m + 8.0f;
-                if (begun && !__any_sync(0xffffffffu, grow)) {
+                const bool any = __any_sync(0xffffffffu, grow);
+                if (begun && !edge && !any) {
                     tmem_st32(tS, pk);
                     tmem_st32(tS + 32, pk + 32);
-                } else {                                  // a larger maximum: O and l to its scale, the weights again
+                } else {                                  // O and l to the scale of a larger maximum; the weights (again)
                     const float f = grow ? ex2(m - top) : 1.0f;
                     if (grow) {
                         m = top;
                         l *= f;
                     }
-                    if (begun) {
+                    if (begun && any) {
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 16) {
                             uint32_t o[16];
@@ -551,7 +645,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    add[0] = add[1] = add[2] = add[3] = 0.0f;
+                    const f32x2 minus = pack2(-base, -base);
+                    add[0] = add[1] = 0;
 #pragma unroll 1
                     for (int c = 0; c < 128; c += 16) {   // P's columns lie behind those of S still to be read
                         uint32_t v[16], w[8];
@@ -559,12 +654,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         tmem_wait_ld();
                         settle16(v);
                         if (edge) hide(v, c);
-                        weigh(v, base, w, add);
+                        weigh(v, minus, w, add, None{});
                         tmem_st8(tS + c / 2, w);
                     }
                     begun = true;
                 }
-                l += (add[0] + add[1]) + (add[2] + add[3]);
+                float a0, a1;
+                unpack2(add2(add[0], add[1]), a0, a1);
+                l += a0 + a1;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
