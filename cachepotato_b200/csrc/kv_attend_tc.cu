@@ -15,7 +15,8 @@
 //                           than 2^8 since the last time: the scale cancels in O / l, and f32 and the
 //                           cache's types hold weights up to 2^8 as well as up to 1. So a tile's
 //                           weights are taken with the maximum at hand, in one pass over S, and only
-//                           if it proves too small are they taken again (a first tile's always).
+//                           if it proves too small are they taken again. (An item's first tile is
+//                           gone over for the maximum first.)
 //           warp 8          producer: q tiles and the ring of K and V tiles, tensor TMA
 //           warp 9          tcgen05.mma: S = q·K^T (both operands in shared memory), O += P·V (P from
 //                           TMEM). While one row tile is in its softmax the other's products run.
@@ -30,7 +31,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "kv_attend.cuh"
 
@@ -38,32 +38,12 @@ namespace cpg {
 
 constexpr int KT_TILE = 128, KT_ROWS = 128;               // positions and rows of an MMA tile
 constexpr int KT_THREADS = 384, KT_PRODUCER = 8, KT_MMA = 9, KT_FIXER = 10;
-constexpr int KT_POLY = 0;                                // pairs in 8 whose exponentials are polynomials
 constexpr int KT_FIXED = 2;                               // units an item's begin and end are worth (see KD_FIXED)
 template <int HD> constexpr int kt_unit() { return KT_TILE * HD * 2; }
 template <int HD> constexpr int kt_units() { return HD == 128 ? 5 : 8; }
 template <int HD> constexpr int kt_smem() { return 1024 + 2 * KT_ROWS * HD * 2 + kt_units<HD>() * kt_unit<HD>(); }
-template <int HD> constexpr int kt_part() { return (2 + HD) * KT_ROWS; }       // floats of a row tile's part: m, l, o
+template <int HD> constexpr int kt_part() { return (2 + HD) * KT_ROWS; }       // floats of a row tile's part: m, l, o (four columns of a row together)
 static_assert(KT_ROWS == 128 && KT_TILE == 128, "tile shapes");
-
-// sum of floor((a·i + b) / m) for 0 <= i < n, by the Euclidean algorithm on (a, m); a, b >= 0, m > 0.
-__device__ long kt_floor_sum(long n, long m, long a, long b) {
-    long sum = 0;
-    for (int step = 0; step < 64 && n > 0; ++step) {
-        const long qa = kv_div(a, m), qb = kv_div(b, m);
-        sum += n * (n - 1) / 2 * qa + n * qb;
-        a -= qa * m;
-        b -= qb * m;
-        const long top = a * n + b;
-        if (top < m) break;
-        n = kv_div(top, m);
-        b = top - n * m;
-        const long x = m;
-        m = a;
-        a = x;
-    }
-    return sum;
-}
 
 // Sequence i in units. Pair p (of row tiles) holds tokens [p·Q, min(len, p·Q + Q)).
 struct KtSeq {
@@ -71,24 +51,18 @@ struct KtSeq {
     int pairs;
     long head_units;                                      // of one cached head
 };
-// units of the first x pairs (of one cached head)
-__device__ long kt_before(const AttendArgs &a, int Q, const KvSeq &s, int pairs, long x) {
-    if (x == 0) return 0;
-    const long whole = min(x, (long)pairs - 1);           // pairs of Q tokens
-    long sum = x * KT_FIXED + kt_floor_sum(whole, KT_TILE, Q, (long)s.p0 + Q - 1) + whole;
-    if (x == pairs) sum += ((long)s.p0 + s.len - 1) / KT_TILE + 1;
-    if (a.window) {                                       // tiles in front of the first token's window
-        const long d = (long)s.p0 - a.window + 1;
-        const long first = d < 0 ? (-d + Q - 1) / Q : 0;
-        if (x > first) sum -= kt_floor_sum(x - first, KT_TILE, Q, d + first * Q);
-    }
-    return sum;
+// position tiles of pair p; with a window, from the first token's on
+__device__ __forceinline__ int kt_tiles(const AttendArgs &a, int Q, const KvSeq &s, int p) {
+    const int lo = a.window ? max(0, s.p0 + p * Q - a.window + 1) : 0;
+    return (s.p0 + min(s.len, p * Q + Q) - 1) / KT_TILE + 1 - lo / KT_TILE;
 }
 __device__ __forceinline__ KtSeq kt_seq(const AttendArgs &a, int Q, int i) {
     KtSeq q;
     q.s = kv_seq(a.b, a.c.P, i);
     q.pairs = (q.s.len + Q - 1) / Q;
-    q.head_units = q.pairs ? kt_before(a, Q, q.s, q.pairs, q.pairs) : 0;
+    q.head_units = 0;
+    // a handful of instructions a pair; a closed form took longer than summing thousands of pairs
+    for (int p = 0; p < q.pairs; ++p) q.head_units += KT_FIXED + kt_tiles(a, Q, q.s, p);
     return q;
 }
 
@@ -104,7 +78,7 @@ struct KtCursor {
     __device__ __forceinline__ void item(const AttendArgs &a, int Q) {
         hi = s.p0 + min(s.len, (pair + 1) * Q);
         lo_t = lo_of(a, pair * Q) / KT_TILE;
-        nt = (hi - 1) / KT_TILE + 1 - lo_t;
+        nt = kt_tiles(a, Q, s, pair);
     }
     __device__ __forceinline__ void next_item(const AttendArgs &a, int Q) {
         kt = -KT_FIXED;
@@ -172,34 +146,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of two numbers on the multiply-add pipe: n = round(x) by adding 1.5 · 2^23, a polynomial of
-// least largest relative error for 2^(x - n) on [-1/2, 1/2] (Remez exchange: 2^-13.7 with degree 3,
-// 2^-18.6 with degree 4, against 2^-9 and 2^-12 of the rounding that follows), n added to the
-// exponent. For x < 128; below 2^-125 it gives 2^-125.
-template <int DEG>
-__device__ __forceinline__ f32x2 ex2_poly2(f32x2 x) {
-    float a, b;
-    unpack2(x, a, b);
-    x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
-    const f32x2 t = add2(x, pack2(12582912.0f, 12582912.0f));
-    const f32x2 r = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
-    f32x2 p;
-    if (DEG == 3) {
-        p = fma2(r, pack2(0.05517167f, 0.05517167f), pack2(0.24261113f, 0.24261113f));
-        p = fma2(r, p, pack2(0.69326097f, 0.69326097f));
-        p = fma2(r, p, pack2(0.99992806f, 0.99992806f));
-    } else {
-        p = fma2(r, pack2(0.0095701021f, 0.0095701021f), pack2(0.055917859f, 0.055917859f));
-        p = fma2(r, p, pack2(0.24024744f, 0.24024744f));
-        p = fma2(r, p, pack2(0.69312179f, 0.69312179f));
-        p = fma2(r, p, pack2(0.99999928f, 0.99999928f));
-    }
-    float p0, p1, t0, t1;
-    unpack2(p, p0, p1);
-    unpack2(t, t0, t1);
-    return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
-                 __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
-}
 
 // Nothing that uses r may be moved before this point (the wait for the loads that fill it).
 __device__ __forceinline__ void settle16(uint32_t *r) {
@@ -223,7 +169,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, asked[NU], fixed[NU], s_full[2], p_full[2], o_full[2], drain;
-    __shared__ long s_scan[KT_THREADS / 32], s_cut[2];
+    __shared__ long s_scan[KT_THREADS / 32], s_cut[2], s_off;
     __shared__ KtCursor s_cur;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_last[2], s_ask[NU][3];     // a V tile to clear: ring slot, its fill's parity, first place
@@ -301,21 +247,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
         }
         if (n <= KT_THREADS && !range(all)) return;
         const long at = u0 - (base + inc - x);
-        if (at >= 0 && at < x) {                          // the pair by bisection
+        if (at >= 0 && at < x) {
             KtCursor c;
             c.seq = c0 + tid;
             c.s = mine.s;
             c.pairs = mine.pairs;
             c.kh = (int)kv_div(at, mine.head_units);
-            const long off = at - c.kh * mine.head_units;
-            int lo = 0, hi = mine.pairs - 1;              // last pair with kt_before <= off
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (kt_before(a, Q, mine.s, mine.pairs, mid) <= off) lo = mid; else hi = mid - 1;
-            }
-            c.pair = lo;
-            c.kt = (int)(off - kt_before(a, Q, mine.s, mine.pairs, lo)) - KT_FIXED;
-            c.item(a, Q);
+            s_off = at - c.kh * mine.head_units;
             s_cur = c;
         }
         before += all;
@@ -326,6 +264,30 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     if (tid == 0) {
         s_cut[0] = cut.each;
         s_cut[1] = cut.more;
+    }
+    if (warp == 0) {                                      // the pair that holds unit s_off, 32 pairs at a time
+        KtCursor c = s_cur;
+        long off = s_off;
+        for (int p0 = 0; p0 < c.pairs; p0 += 32) {
+            const int p = p0 + lane, mine = p < c.pairs ? KT_FIXED + kt_tiles(a, Q, c.s, p) : 0;
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            const int all = __shfl_sync(0xffffffffu, inc, 31);
+            if (off < all) {
+                if (off >= inc - mine && off < inc) {
+                    c.pair = p;
+                    c.kt = (int)off - (inc - mine) - KT_FIXED;
+                    c.item(a, Q);
+                    s_cur = c;
+                }
+                break;
+            }
+            off -= all;
+        }
     }
     if (warp == KT_MMA) {                                 // all of TMEM
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
@@ -558,81 +520,45 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                 const bool edge = j0 + KT_TILE > cur.s.p0 + rt.t0 + 1 || (a.window && j0 < rt.hi - a.window);
                 const int top_j = p - j0, bottom_j = a.window ? top_j - a.window : -1;
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // scores of 16 columns from c that the row does not see
                 auto hide = [&](uint32_t *v, int c) {
+                    const int up = min(max(top_j + 1 - c, 0), 16), dn = min(max(bottom_j + 1 - c, 0), 16);
+                    const uint32_t seen = ((1u << up) - 1u) & ~((1u << dn) - 1u);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (c + e > top_j || c + e <= bottom_j) v[e] = 0xff800000u;
+                        if (!(seen >> e & 1u)) v[e] = 0xff800000u;
                 };
-                // weights of 16 scores -> 8 packed pairs; their sum added to `add`. POLY of the 8 pairs
-                // go to the multiply-add pipe
+                // weights of 16 scores -> 8 packed pairs; their sum added to `add`
                 const f32x2 scale22 = pack2(a.scale2, a.scale2);
-                auto weigh = [&](const uint32_t *v, f32x2 minus, uint32_t *pk, f32x2 (&add)[2], auto poly) {
+                auto weigh = [&](const uint32_t *v, f32x2 minus, uint32_t *pk, f32x2 (&add)[2]) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        f32x2 x = fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale22, minus);
+                        const f32x2 x = fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale22, minus);
                         float e0, e1;
-                        if ((e + 1) * decltype(poly)::value / 8 > e * decltype(poly)::value / 8) {
-                            x = ex2_poly2<HALF ? 4 : 3>(x);
-                            unpack2(x, e0, e1);
-                        } else {
-                            unpack2(x, e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                            x = pack2(e0, e1);
-                        }
-                        add[e & 1] = add2(add[e & 1], x);
+                        unpack2(x, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                        add[e & 1] = add2(add[e & 1], pack2(e0, e1));
                         uint32_t w[1];
                         split_pair<HALF, 1>(e0, e1, w);
                         pk[e] = w[0];
                     }
                 };
-                using None = std::integral_constant<int, 0>;
-                using Some = std::integral_constant<int, KT_POLY>;
                 auto largest = [&](const uint32_t *v) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 2)
                         mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
                 };
-                f32x2 add[2] = {0, 0};
-                uint32_t pk[64];                          // kept until m has proved large enough
-                if (begun && !edge) {
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    const f32x2 minus = pack2(-base, -base);
-                    uint32_t s[2][16];
-                    tmem_ld16_nowait(tS, s[0]);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {         // 16 columns while the next 16 are on their way
-                        uint32_t *const v = s[c & 1];
-                        tmem_wait_ld();
-                        settle16(v);
-                        if (c < 7) tmem_ld16_nowait(tS + 16 * (c + 1), s[(c + 1) & 1]);
-                        largest(v);
-                        weigh(v, minus, pk + 8 * c, add, Some{});
-                    }
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < 128; c += 16) {
-                        uint32_t v[16];
-                        tmem_ld16_nowait(tS + c, v);
-                        tmem_wait_ld();
-                        settle16(v);
-                        if (edge) hide(v, c);
-                        largest(v);
-                    }
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
-                const bool grow = top > m + 8.0f;
-                const bool any = __any_sync(0xffffffffu, grow);
-                if (begun && !edge && !any) {
-                    tmem_st32(tS, pk);
-                    tmem_st32(tS + 32, pk + 32);
-                } else {                                  // O and l to the scale of a larger maximum; the weights (again)
+                // O and l to the scale of a larger maximum
+                auto raise = [&](float top) {
+                    const bool grow = top > m + 8.0f;
+                    if (!__any_sync(0xffffffffu, grow)) return false;
                     const float f = grow ? ex2(m - top) : 1.0f;
                     if (grow) {
                         m = top;
                         l *= f;
                     }
-                    if (begun && any) {
+                    if (begun) {                          // O holds sums (an item's first product sets it)
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 16) {
                             uint32_t o[16];
@@ -644,6 +570,49 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                             tmem_st16(tO + c, o);
                         }
                     }
+                    return true;
+                };
+                auto top_of = [&]() { return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2; };
+                if (!begun) {                             // nothing is known of the maximum yet
+                    uint32_t s[2][32];
+                    tmem_ld32_nowait(tS, s[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t *const v = s[c & 1];
+                        tmem_wait_ld();
+                        settle32(v);
+                        if (c < 3) tmem_ld32_nowait(tS + 32 * (c + 1), s[(c + 1) & 1]);
+                        if (edge) {
+                            hide(v, 32 * c);
+                            hide(v + 16, 32 * c + 16);
+                        }
+                        largest(v);
+                        largest(v + 16);
+                    }
+                    raise(top_of());
+                }
+                f32x2 add[2] = {0, 0};
+                uint32_t pk[64];                          // kept until m has proved large enough
+                {
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    const f32x2 minus = pack2(-base, -base);
+                    uint32_t s[2][16];
+                    tmem_ld16_nowait(tS, s[0]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {         // 16 columns while the next 16 are on their way
+                        uint32_t *const v = s[c & 1];
+                        tmem_wait_ld();
+                        settle16(v);
+                        if (c < 7) tmem_ld16_nowait(tS + 16 * (c + 1), s[(c + 1) & 1]);
+                        if (edge) hide(v, 16 * c);
+                        largest(v);
+                        weigh(v, minus, pk + 8 * c, add);
+                    }
+                }
+                if (!raise(top_of())) {
+                    tmem_st32(tS, pk);
+                    tmem_st32(tS + 32, pk + 32);
+                } else {                                  // rarely: the weights again, with the new maximum
                     const float base = m == -INFINITY ? 0.0f : m;
                     const f32x2 minus = pack2(-base, -base);
                     add[0] = add[1] = 0;
@@ -654,11 +623,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         tmem_wait_ld();
                         settle16(v);
                         if (edge) hide(v, c);
-                        weigh(v, minus, w, add, None{});
+                        weigh(v, minus, w, add);
                         tmem_st8(tS + c / 2, w);
                     }
-                    begun = true;
                 }
+                begun = true;
                 float a0, a1;
                 unpack2(add2(add[0], add[1]), a0, a1);
                 l += a0 + a1;
@@ -723,16 +692,21 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     for (gs = 2; gs * gs < np;) ++gs;
                 const int ng = (np + gs - 1) / gs, gi = pi / gs, n_in = min(gs, np - gi * gs);
                 auto slot_of = [&](int k) { return k == 0 ? 2 * b0 + 1 : 2 * (b0 + k); };
-                auto part = [&](int k) { return a.part + ((size_t)slot_of(k) * 2 + x) * kt_part<HD>() + row; };
+                auto part = [&](int k) { return a.part + ((size_t)slot_of(k) * 2 + x) * kt_part<HD>(); };
+                auto put16 = [&](float *to, int c, const float *v) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        __stcg(reinterpret_cast<float4 *>(to + 2 * KT_ROWS) + (c / 4 + e) * KT_ROWS + row,
+                               make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
+                };
                 float *to = part(pi);
-                __stcg(to, m);
-                __stcg(to + KT_ROWS, l);
+                __stcg(to + row, m);
+                __stcg(to + KT_ROWS + row, l);
 #pragma unroll 2
                 for (int c = 0; c < HD; c += 16) {
                     float v[16];
                     load16(c, v);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) __stcg(to + (2 + c + e) * KT_ROWS, v[e]);
+                    put16(to, c, v);
                 }
                 // parts first, first + step, ... (count of them), joined by the last of their blocks:
                 // into the first one's place, or (last) into out
@@ -751,37 +725,52 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     if (!mine) return false;
                     float M = -INFINITY, L = 0.0f;
 #pragma unroll 4
-                    for (int k = 0; k < count; ++k) M = fmaxf(M, __ldcg(part(firstp + k * step)));
+                    for (int k = 0; k < count; ++k) M = fmaxf(M, __ldcg(part(firstp + k * step) + row));
                     const float bs = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
                     for (int k = 0; k < count; ++k)
-                        L = fmaf(ex2(__ldcg(part(firstp + k * step)) - bs), __ldcg(part(firstp + k * step) + KT_ROWS), L);
+                        L = fmaf(ex2(__ldcg(part(firstp + k * step) + row) - bs), __ldcg(part(firstp + k * step) + KT_ROWS + row), L);
                     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
                     float *put = part(firstp);
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
-                        float v[16];
+                    for (int c = 0; c < HD; c += 32) {
+                        float v[32];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = 0.0f;
-#pragma unroll 2
-                        for (int k = 0; k < count; ++k) {
-                            const float *src = part(firstp + k * step);
-                            const float w = ex2(__ldcg(src) - bs);
-                            float y[16];
+                        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+                        for (int k = 0; k < count; k += 2) {              // two parts' columns in flight
+                            float4 y[2][8];
+                            float w[2];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) y[e] = __ldcg(src + (2 + c + e) * KT_ROWS);
+                            for (int z = 0; z < 2; ++z) {
+                                const float *src = part(firstp + min(k + z, count - 1) * step);
+                                w[z] = __ldcg(src + row);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = fmaf(w, y[e], v[e]);
+                                for (int e = 0; e < 8; ++e)
+                                    y[z][e] = __ldcg(reinterpret_cast<const float4 *>(src + 2 * KT_ROWS) + (c / 4 + e) * KT_ROWS + row);
+                            }
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                const float f = k + z < count ? ex2(w[z] - bs) : 0.0f;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    v[4 * e] = fmaf(f, y[z][e].x, v[4 * e]);
+                                    v[4 * e + 1] = fmaf(f, y[z][e].y, v[4 * e + 1]);
+                                    v[4 * e + 2] = fmaf(f, y[z][e].z, v[4 * e + 2]);
+                                    v[4 * e + 3] = fmaf(f, y[z][e].w, v[4 * e + 3]);
+                                }
+                            }
                         }
-                        if (last) write16(c, v, inv);
-                        else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) __stcg(put + (2 + c + e) * KT_ROWS, v[e]);
+                        if (last) {
+                            write16(c, v, inv);
+                            write16(c + 16, v + 16, inv);
+                        } else {
+                            put16(put, c, v);
+                            put16(put, c + 16, v + 16);
                         }
                     }
                     if (!last) {
-                        __stcg(put, M);
-                        __stcg(put + KT_ROWS, L);
+                        __stcg(put + row, M);
+                        __stcg(put + KT_ROWS + row, L);
                     }
                     return true;
                 };
