@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
                 const long p = (long)p0 + (t - a0);
                 pos = (int)min(p, 0x7fffffffl);
                 const int at = pos / a.c.P;
-                const bool inside = p <= 0x7fffffffl && at < a.b.max_pages;
+                const bool inside = p < 0x7fff0000l && at < a.b.max_pages;
                 if (inside) page = a.b.pages[(size_t)i * a.b.table_stride + at];
                 if (page < 0 || page >= a.c.n_pages) {
                     page = -1;
@@ -431,6 +431,7 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
                 n_heads, kv->v.KV);
     CPG_REQUIRE(scale > 0.0f && isfinite(scale), "%s: scale %g must be positive", fn, (double)scale);
     CPG_REQUIRE(window >= 0, "%s: window %d", fn, window);
+    CPG_REQUIRE((long)r.T * n_heads <= 0x7fff0000l, "%s: %d rows of %d heads", fn, r.T, n_heads);
     if (r.T == 0 || r.n == 0) return CPG_OK;
     rc = rows_ok(fn, "q", q, q_stride, n_heads, kv->hd, type);
     if (!rc) rc = rows_ok(fn, "out", out, out_stride, n_heads, kv->hd, type);

@@ -90,7 +90,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int P, int i) {
     s.r0 = max(a, 0);
     s.len = max(0, min(e, b.T) - s.r0);
     s.bad = a < 0 || e < a || e > b.T || s.p0 < 0;
-    const long cap = (long)b.max_pages * P;
+    const long cap = min((long)b.max_pages * P, 0x7fff0000l);   // positions and tile ends stay in 32 bits
     if (s.p0 < 0) s.len = 0;
     if ((long)s.p0 + s.len > cap) {
         s.len = (int)max(0l, cap - s.p0);

@@ -93,51 +93,59 @@ constexpr int KD_JOIN = 24;                              // parts of one join, a
 template <int HD> constexpr int kd_buf() { return 3 * HD / 16 * 512; }
 template <int HD> constexpr int kd_smem() { return 1008 + KD_RING + kd_buf<HD>() + KD_JOIN * 2 * KD_ROWS * 4; }
 
-// Sequence i's units: KV · row tiles · (KD_FIXED + position tiles), the same for each of its items.
+// Sequence i's units: for each row tile, KV · (KD_FIXED + the position tiles its rows see).
 // Beginning and ending an item takes a block as long as some three tiles (4 us against 1.4 us for 64
 // bf16 positions), so an item counts for KD_FIXED tiles more than it has: without them the blocks
 // that end one item and begin the next finish last (128K positions, one row: 62 us against 53 us).
 constexpr int KD_FIXED = 3;
 struct KdSeq {
     KvSeq s;
-    int rt, nt, lo_t;
+    int rt;                          // row tiles
     long units;
+};
+// Row tile r of a sequence: its (row, head) pairs from r0, nr of them, and the positions they see.
+struct KdRows {
+    int r0, nr, lo, hi, lo_t, nt;
+    __device__ __forceinline__ KdRows() {}
+    __device__ __forceinline__ KdRows(const AttendArgs &a, int G, const KvSeq &s, int r) {
+        r0 = r * KD_ROWS;
+        nr = min(KD_ROWS, s.len * G - r0);
+        lo = a.window ? max(0, s.p0 + r0 / G - a.window + 1) : 0;
+        hi = s.p0 + (r0 + nr - 1) / G + 1;
+        lo_t = lo / KD_TILE;
+        nt = (hi + KD_TILE - 1) / KD_TILE - lo_t;
+    }
 };
 __device__ __forceinline__ KdSeq kd_seq(const AttendArgs &a, int G, int i) {
     KdSeq q;
     q.s = kv_seq(a.b, a.c.P, i);
     q.rt = (int)(((long)q.s.len * G + KD_ROWS - 1) / KD_ROWS);
-    q.lo_t = a.window ? max(0, q.s.p0 - a.window + 1) / KD_TILE : 0;
-    q.nt = q.s.len ? (q.s.p0 + q.s.len + KD_TILE - 1) / KD_TILE - q.lo_t : 0;
-    q.units = q.nt ? (long)a.c.KV * q.rt * (q.nt + KD_FIXED) : 0;
+    long tiles = 0;
+    for (int r = 0; r < q.rt; ++r) tiles += KD_FIXED + KdRows(a, G, q.s, r).nt;
+    q.units = a.c.KV * tiles;
     return q;
 }
 
 // A place in the order of units: item (seq, row tile, cached head), position tile.
 struct KdCursor {
-    int seq, sub, kt;                // sub = row tile · KV + cached head; kt from -KD_FIXED
-    KdSeq q;
-    int r0, nr, lo, hi;              // the row tile: first (row, head) pair, their number, positions seen
-    __device__ __forceinline__ void item(const AttendArgs &a, int G) {
-        r0 = sub / a.c.KV * KD_ROWS;
-        nr = min(KD_ROWS, q.s.len * G - r0);
-        lo = a.window ? max(0, q.s.p0 + r0 / G - a.window + 1) : 0;
-        hi = q.s.p0 + (r0 + nr - 1) / G + 1;
-    }
+    int seq, rt, kh, kt;             // kt from -KD_FIXED
+    KvSeq s;
+    int n_rt;
+    KdRows r;
     __device__ __forceinline__ void next_item(const AttendArgs &a, int G) {
         kt = -KD_FIXED;
-        if (++sub < q.rt * a.c.KV) {
-            item(a, G);
-            return;
+        if (++kh < a.c.KV) return;
+        kh = 0;
+        if (++rt == n_rt) {
+            rt = 0;
+            do {
+                if (++seq >= a.b.n) return;
+                s = kv_seq(a.b, a.c.P, seq);
+            } while (s.len == 0);
+            n_rt = (int)(((long)s.len * G + KD_ROWS - 1) / KD_ROWS);
         }
-        sub = 0;
-        do {
-            if (++seq >= a.b.n) return;
-            q = kd_seq(a, G, seq);
-        } while (q.units == 0);
-        item(a, G);
+        r = KdRows(a, G, s, rt);
     }
-    __device__ __forceinline__ int head(const AttendArgs &a) const { return sub % a.c.KV; }
 };
 
 template <typename TI, typename TC, int HD>
@@ -155,8 +163,8 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t full[NU], empty[NU];
     __shared__ long s_scan[KD_WARPS + 1], s_off;
-    __shared__ KdSeq s_item;
-    __shared__ int s_seq, s_last, s_abort;
+    __shared__ KdCursor s_cur;
+    __shared__ int s_last, s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.H / a.c.KV;
     if (tid == 0) {
@@ -226,21 +234,49 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         }
         if (n <= KD_THREADS && !range(all)) return;
         if (c0 + tid < n && u0 >= base + inc - x && u0 < base + inc) {
-            s_seq = c0 + tid;
+            KdCursor c;
+            c.seq = c0 + tid;
+            c.s = mine.s;
+            c.n_rt = mine.rt;
             s_off = u0 - (base + inc - x);
-            s_item = mine;
+            s_cur = c;
         }
         before += all;
         __syncthreads();
         if (u0 < before) break;
     }
     if (u0 >= u1) return;                                 // no sequences at all
-    KdCursor cur;
-    cur.seq = s_seq;
-    cur.q = s_item;
-    cur.sub = (int)kv_div(s_off, cur.q.nt + KD_FIXED);
-    cur.kt = (int)(s_off - (long)cur.sub * (cur.q.nt + KD_FIXED)) - KD_FIXED;
-    cur.item(a, G);
+    if (warp == 0) {                                      // the row tile that holds unit s_off, 32 at a time
+        KdCursor c = s_cur;
+        long off = s_off;
+        for (int r0 = 0; r0 < c.n_rt; r0 += 32) {
+            const int r = r0 + lane;
+            int each = 0;
+            if (r < c.n_rt) {
+                c.r = KdRows(a, G, c.s, r);
+                each = KD_FIXED + c.r.nt;
+            }
+            long inc = (long)each * a.c.KV;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            const long all = __shfl_sync(0xffffffffu, inc, 31), from = inc - (long)each * a.c.KV;
+            if (off < all) {
+                if (off >= from && off < inc) {
+                    c.rt = r;
+                    c.kh = (int)(off - from) / each;
+                    c.kt = (int)(off - from) - c.kh * each - KD_FIXED;
+                    s_cur = c;
+                }
+                break;
+            }
+            off -= all;
+        }
+    }
+    __syncthreads();
+    KdCursor cur = s_cur;
     volatile int *const abort_flag = &s_abort;
 
     if (warp == KD_WARPS) {
@@ -254,7 +290,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                 ++cur.kt;
                 continue;
             }
-            const int j0 = (cur.q.lo_t + cur.kt) * KD_TILE;
+            const int j0 = (cur.r.lo_t + cur.kt) * KD_TILE;
             const int boxes = groups * PARTS;
             int page[2], place[2];                        // boxes lane, lane + 32 (at most 8 groups of 4)
 #pragma unroll
@@ -262,7 +298,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                 const int bx = lane + 32 * x, j = j0 + bx / PARTS * a.box;
                 page[x] = a.c.n_pages;                    // outside the pool: zeros
                 place[x] = 0;
-                if (bx < boxes && j < cur.hi && j + a.box > cur.lo) {
+                if (bx < boxes && j < cur.r.hi && j + a.box > cur.r.lo) {
                     const int pg = j / a.c.P;
                     const int id = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
                     if (id >= 0 && id < a.c.n_pages) page[x] = id;
@@ -286,7 +322,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                     const int bx = lane + 32 * x, part = bx % PARTS;
                     if (bx < boxes)
                         tma_load_4d(ring + slot * UNIT + part * (KD_TILE * 128) + bx / PARTS * a.box * 128, half ? &tm_v : &tm_k,
-                                    part * (128 / ES), place[x], cur.head(a), page[x], &full[slot]);
+                                    part * (128 / ES), place[x], cur.kh, page[x], &full[slot]);
                 }
                 if (++slot == NU) {
                     slot = 0;
@@ -294,7 +330,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                 }
             }
             if (stop) break;
-            if (++cur.kt == cur.q.nt && u + 1 < u1) cur.next_item(a, G);
+            if (++cur.kt == cur.r.nt && u + 1 < u1) cur.next_item(a, G);
         }
         if (stop) {                                       // copies in flight land before the block may end
             for (int i = 0; i < NU; ++i) {
@@ -321,16 +357,16 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             if (u >= u1) break;                           // its first tile is the next block's
         }
         {                                                 // an item: its rows of q, empty sums
-            const int kh = cur.head(a);
+            const int kh = cur.kh;
             float f[2][F32I ? KS : 1][4];
             float up[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int rr = cur.r0 + g + 8 * r;
-                const bool live = g + 8 * r < cur.nr;
+                const int rr = cur.r.r0 + g + 8 * r;
+                const bool live = g + 8 * r < cur.r.nr;
                 const int tok = rr / G;
-                p_row[r] = live ? cur.q.s.p0 + tok : cur.hi - 1;
-                const TI *src = (const TI *)a.q + (size_t)(cur.q.s.r0 + tok) * a.q_stride + (size_t)(kh * G + rr - tok * G) * HD;
+                p_row[r] = live ? cur.s.p0 + tok : cur.r.hi - 1;
+                const TI *src = (const TI *)a.q + (size_t)(cur.s.r0 + tok) * a.q_stride + (size_t)(kh * G + rr - tok * G) * HD;
                 sc[r] = a.scale2;
                 up[r] = 1.0f;
                 if constexpr (!F32I) {
@@ -399,11 +435,11 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
             for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         }
-        const int n_here = (int)min((long)(cur.q.nt - cur.kt), u1 - u);          // this block's tiles of it
-        int j0 = (cur.q.lo_t + cur.kt) * KD_TILE + warp * KD_KEYS;
+        const int n_here = (int)min((long)(cur.r.nt - cur.kt), u1 - u);          // this block's tiles of it
+        int j0 = (cur.r.lo_t + cur.kt) * KD_TILE + warp * KD_KEYS;
 #pragma unroll 1
         for (int left = n_here; left > 0; --left, j0 += KD_TILE) {
-            const bool active = j0 < cur.hi && j0 + KD_KEYS > cur.lo;
+            const bool active = j0 < cur.r.hi && j0 + KD_KEYS > cur.r.lo;
             float s[2][4], c[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {            // K, then V
@@ -473,8 +509,8 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[n][e] = (big[n][0][e] + big[n][1][e]) + low[n][e];
                     }
-                    const int span = (cur.nr - 1) / G + 1;    // positions between the tile's rows, at most
-                    if (j0 + KD_KEYS > cur.hi - span || (a.window && j0 < cur.lo + span)) {
+                    const int span = (cur.r.nr - 1) / G + 1;    // positions between the tile's rows, at most
+                    if (j0 + KD_KEYS > cur.r.hi - span || (a.window && j0 < cur.r.lo + span)) {
                         // some row of the tile does not see all 16
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
@@ -527,9 +563,9 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
                         const int j = j0 + 2 * t + (y & 1) + 8 * (y >> 1);
-                        hide[y] = j >= cur.hi || j < cur.lo;
+                        hide[y] = j >= cur.r.hi || j < cur.r.lo;
                     }
-                    const bool any = j0 + KD_KEYS > cur.hi || j0 < cur.lo;
+                    const bool any = j0 + KD_KEYS > cur.r.hi || j0 < cur.r.lo;
                     // f32 rows: o = o·c + sum, rounded
                     auto add_to = [&](float (&to)[4], const float (&sum)[4]) {
 #pragma unroll
@@ -675,7 +711,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         }
 
         // ---- who else has a part of it: the item's tiles are units [ua, ue), blocks b0..b1
-        const long ua = u - cur.kt, ue = ua + cur.q.nt;
+        const long ua = u - cur.kt, ue = ua + cur.r.nt;
         u += n_here;
         const int b0 = cut.owner(ua), b1 = cut.owner(ue - 1);
         bool write = b0 == b1;
@@ -731,7 +767,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                         for (int i = 0; i < NQT; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[x][i][e] = e < 2 || cur.nr > 8 ? __ldcg(src + (4 * i + e) * 32) : 0.0f;
+                            for (int e = 0; e < 4; ++e) v[x][i][e] = e < 2 || cur.r.nr > 8 ? __ldcg(src + (4 * i + e) * 32) : 0.0f;
                     }
                     if (k0 == 0) {
                         named_bar_sync(1, KD_WARPS * 32);
@@ -760,12 +796,12 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             }
         }
         if (write) {
-            const int kh = cur.head(a);
+            const int kh = cur.kh;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if (g + 8 * r >= cur.nr) continue;
-                const int rr = cur.r0 + g + 8 * r, tok = rr / G;
-                TI *dst = (TI *)a.out + (size_t)(cur.q.s.r0 + tok) * a.out_stride + (size_t)(kh * G + rr - tok * G) * HD;
+                if (g + 8 * r >= cur.r.nr) continue;
+                const int rr = cur.r.r0 + g + 8 * r, tok = rr / G;
+                TI *dst = (TI *)a.out + (size_t)(cur.s.r0 + tok) * a.out_stride + (size_t)(kh * G + rr - tok * G) * HD;
                 const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
                 if constexpr (!F32C) {
 #pragma unroll

@@ -47,7 +47,7 @@ class KVBatch:
         _require(q_start.shape[0] == n + 1 and pages.shape[0] == n,
                  f"{n} sequences need {n + 1} starts and {n} table rows, got {q_start.shape[0]} and {pages.shape[0]}")
         _require(rows >= 0 and max_new >= 0, "rows and max_new must not be negative")
-        self.device, self.n_seqs, self.rows = dev, n, int(rows)
+        self.device, self.index, self.n_seqs, self.rows = dev, q_start.get_device(), n, int(rows)
         wide = pages.shape[1]
         stride = pages.stride(0) if n > 1 else wide
         self._c = KvRows(n, self.rows, q_start.data_ptr(), pos0.data_ptr(), pages.data_ptr(), stride, wide, int(max_new))
@@ -69,6 +69,7 @@ class KVCache:
                  and all(n == 1 or a == b for n, a, b in zip(k_pool.shape, k_pool.stride(), v_pool.stride())),
                  "k_pool and v_pool must agree in shape, strides, type and device")
         self.k_pool, self.v_pool, self.device = k_pool, v_pool, k_pool.device
+        self._index = k_pool.get_device()
         self.n_pages, self.page_size, self.n_kv, self.head_dim = k_pool.shape
         self.dtype, self._type = k_pool.dtype, _TYPES[k_pool.dtype]
         sp, st, sh, _ = k_pool.stride()
@@ -90,22 +91,20 @@ class KVCache:
         with torch.cuda.stream(stream):
             return torch.zeros(n, dtype=torch.uint8, device=self.device)
 
-    def _rows(self, t, what: str, batch: KVBatch, heads: int | None):
+    def _rows(self, t, what: str, rows: int, heads: int | None):
         """Row stride of t (rows, heads, head_dim) after its checks."""
-        if not (t.dim() == 3 and t.shape[0] == batch.rows and t.shape[2] == self.head_dim
-                and (heads is None or t.shape[1] == heads)):
-            raise _lib.CpgError(_lib.CPG_EINVAL, f"{what} of shape {tuple(t.shape)}: ({batch.rows}, "
-                                f"{'heads' if heads is None else heads}, {self.head_dim}) expected")
-        stride = t.stride()
-        if t.device != self.device or t.dtype not in _TYPES or stride[2] != 1 or (
-                t.shape[1] > 1 and stride[1] != self.head_dim):
-            raise _lib.CpgError(_lib.CPG_EINVAL, f"{what} must be on {self.device}, f32 or the cache's type, the heads "
-                                "of a row dense")
-        return stride[0] if batch.rows > 1 else t.shape[1] * self.head_dim
+        shape, stride, hd = t.shape, t.stride(), self.head_dim
+        if len(shape) == 3 and shape[0] == rows and shape[2] == hd and stride[2] == 1 and (
+                shape[1] == heads or heads is None) and (stride[1] == hd or shape[1] == 1) and (
+                t.get_device() == self._index and t.dtype in _TYPES):
+            return stride[0] if rows > 1 else shape[1] * hd
+        raise _lib.CpgError(_lib.CPG_EINVAL, f"{what} of shape {tuple(shape)}, strides {stride}, {t.dtype} on {t.device}: "
+                            f"({rows}, {'heads' if heads is None else heads}, {hd}) of f32 or the cache's type, the heads "
+                            f"of a row dense, on {self.device}")
 
     def _call(self, stream, fn, *args):
-        index = self.device.index
-        if torch.cuda.current_device() != index:
+        index = self._index
+        if torch._C._cuda_getDevice() != index:
             with torch.cuda.device(index):
                 return self._call(stream, fn, *args)
         s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
@@ -117,20 +116,20 @@ class KVCache:
         """Keys and values of the batch's rows into their pages; returns the queries, normed and
         rotated like the keys (q_out: written there; may be q). q (rows, n_heads, head_dim) or None,
         k and v (rows, n_kv, head_dim); q_norm, k_norm f32 gains (head_dim) or None."""
-        _require(batch.device == self.device, "the batch and the cache must be on one device")
-        ks, vs = self._rows(k, "k", batch, self.n_kv), self._rows(v, "v", batch, self.n_kv)
+        _require(batch.index == self._index, "the batch and the cache must be on one device")
+        ks, vs = self._rows(k, "k", batch.rows, self.n_kv), self._rows(v, "v", batch.rows, self.n_kv)
         dt = k.dtype
         heads = qs = os_ = 0
         if q is not None:
-            qs, heads = self._rows(q, "q", batch, None), q.shape[1]
+            qs, heads = self._rows(q, "q", batch.rows, None), q.shape[1]
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            os_ = self._rows(q_out, "q_out", batch, heads)
+            os_ = self._rows(q_out, "q_out", batch.rows, heads)
             _require(q.dtype == dt and q_out.dtype == dt, "q, k, v and q_out must have one type")
         _require(v.dtype == dt, "q, k, v and q_out must have one type")
         for g in (q_norm, k_norm):
-            _require(g is None or (g.dtype == torch.float32 and g.shape == (self.head_dim,) and g.is_contiguous()
-                                   and g.device == self.device), "gains are f32 (head_dim) on the cache's device")
+            _require(g is None or (g.dtype is torch.float32 and g.shape == (self.head_dim,) and g.is_contiguous()
+                                   and g.get_device() == self._index), "gains are f32 (head_dim) on the cache's device")
         self._call(stream, self._append, batch._ref, _TYPES[dt], heads, None if q is None else q.data_ptr(), qs,
                    k.data_ptr(), ks, v.data_ptr(), vs, None if q_norm is None else q_norm.data_ptr(),
                    None if k_norm is None else k_norm.data_ptr(), eps, None if q is None else q_out.data_ptr(), os_)
@@ -140,16 +139,16 @@ class KVCache:
         """Attention of the batch's rows over their sequences' cached positions (their own included,
         so append first). q (rows, n_heads, head_dim) f32 or of the cache's type; returns out of q's
         shape and type (written there if given; may be q). scale: head_dim ** -0.5 unless given."""
-        _require(batch.device == self.device, "the batch and the cache must be on one device")
-        qs = self._rows(q, "q", batch, None)
+        _require(batch.index == self._index, "the batch and the cache must be on one device")
+        qs = self._rows(q, "q", batch.rows, None)
         heads = q.shape[1]
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        os_ = self._rows(out, "out", batch, heads)
+        os_ = self._rows(out, "out", batch.rows, heads)
         _require(out.dtype == q.dtype, "out and q must have one type")
         if ws is None:
             ws = self.workspace(heads, stream)
-        _require(ws.device == self.device and ws.is_contiguous(), "the workspace must be dense, on the cache's device")
+        _require(ws.get_device() == self._index and ws.is_contiguous(), "the workspace must be dense, on the cache's device")
         self._call(stream, self._attend, batch._ref, _TYPES[q.dtype], heads, q.data_ptr(), qs, out.data_ptr(), os_,
                    self._scale if scale is None else scale, window, ws.data_ptr(), ws.numel() * ws.element_size())
         return out

@@ -299,6 +299,74 @@ def test_attend_scale_and_in_place():
         assert cache.attend(b.device(50), q, out=q) is q and torch.equal(q, want)
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 100])
+def test_pages_in_front_of_the_window_may_be_gone(rt, ct, new):
+    """Positions no row sees any more are not looked up: their table entries may be anything."""
+    from cachepotato_b200.kv import KVCache
+    window, page = 70, 16
+    b = R.Batch([(new, 500), (new, 3)], page, 6)
+    kp, vp = R.pools(b, 2, 128, TYPES[ct], 7)
+    q = rows((b.rows, 8, 128), TYPES[rt], 8)
+    cache, batch = KVCache(kp, vp, rope_dim=0), b.device(new)
+    want = cache.attend(batch, q, window=window)
+    gone = (500 - window + 1) // page                             # pages that end before the first row's window
+    batch.pages[0, :gone] = torch.tensor([-1, b.n_pages, -7] * gone, dtype=torch.int32, device="cuda")[:gone]
+    assert torch.equal(cache.attend(batch, q, window=window), want)
+    cache.check()
+
+
+@pytest.mark.parametrize("rt,ct", COMBOS)
+def test_one_pool_for_keys_and_values(rt, ct):
+    """Keys and values side by side in one tensor, part of a wider one: strides of no dense layout."""
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(1, 90), (40, 33), (0, 4), (1, 0)], 16, 3, pad=1)
+    big = torch.full((b.n_pages, 3, 16, 4, 2, 64), 9.0, dtype=TYPES[ct], device="cuda")
+    kp, vp = big[:, 0, :, 1:3, 0], big[:, 2, :, 1:3, 0]           # (pages, places, 2 of 4 heads, 64)
+    for p, s in ((kp, 4), (vp, 5)):
+        p.copy_(rows(p.shape, TYPES[ct], s))
+    rest = torch.ones_like(big, dtype=torch.bool)
+    rest[:, 0, :, 1:3, 0] = rest[:, 2, :, 1:3, 0] = False
+    qkv = rows((b.rows, 12, 64), TYPES[rt], 6)
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    cache = KVCache(kp, vp, rope_theta=1e4)
+    want = R.append(b, q.cpu(), k.cpu(), v.cpu(), kp, vp, None, None, 0.0, 64, 1e4)
+    qr = cache.append(b.device(40), q, k, v)
+    amp = lambda w: torch.hypot(w, torch.cat([w[..., 32:], w[..., :32]], -1))
+    close(kp, want[1], half_step(TYPES[ct]) * want[1].abs() * (1 + 2 ** -8) + 32 * U * amp(want[1]) + tiny(TYPES[ct]), "keys")
+    close(vp, want[2], half_step(TYPES[ct]) * want[2].abs() + tiny(TYPES[ct]), "values")
+    assert bool((big[rest] == 9.0).all())
+    qr[int(b.start[-1]):] = 0
+    ref, size = R.attend(b, qr, kp, vp, 64 ** -0.5, 0)
+    close(cache.attend(b.device(40), qr), ref, attend_tol(b, ref, size, vp, TYPES[rt]), "attend")
+    cache.check()
+
+
+@pytest.mark.parametrize("H,KV", [(100, 1), (130, 1), (256, 2)])
+@pytest.mark.parametrize("rt,ct", [("f32", "f16"), ("bf16", "bf16")])
+def test_attend_very_many_heads_to_a_cached_one(H, KV, rt, ct):
+    check_attend([(1, 200), (9, 33), (3, 0)], 16, H, KV, 64, TYPES[rt], TYPES[ct], max_new=9)
+
+
+@pytest.mark.parametrize("rt,ct", [("f32", "f32"), ("bf16", "bf16")])
+def test_rows_in_front_of_the_first_sequence(rt, ct):
+    """q_start need not begin at zero: earlier rows belong to nobody."""
+    from cachepotato_b200.kv import KVBatch, KVCache
+    for new in (1, 60):
+        b = R.Batch([(new, 20), (1, 70)], 16, 3)
+        kp, vp = R.pools(b, 2, 64, TYPES[ct], 4)
+        cache, q = KVCache(kp, vp), rows((b.rows + 5, 4, 64), TYPES[rt], 5)
+        plain, moved = b.device(new), b.device(new)
+        moved = KVBatch(plain.q_start + 5, plain.pos0, plain.pages, rows=b.rows + 5, max_new=new)
+        out = torch.full_like(q, 7.0)
+        cache.attend(moved, q, out=out)
+        assert bool((out[:5] == 7.0).all()) and torch.equal(out[5:], cache.attend(plain, q[5:].contiguous()))
+        got = cache.append(moved, q, q[:, :2], q[:, 2:], q_out=torch.full_like(q, 7.0))
+        assert bool((got[:5] == 7.0).all())
+        assert torch.equal(got[5:], cache.append(plain, q[5:].contiguous(), q[5:, :2], q[5:, 2:]))
+        cache.check()
+
+
 def test_attend_bad_tables_touch_nothing():
     """Page ids outside the pool and positions past the table: reported once, the other sequences' rows
     right, later calls unaffected."""
