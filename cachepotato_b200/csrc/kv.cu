@@ -248,7 +248,7 @@ int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &
                      cudaStream_t s);
 int tensor_map(CUtensorMap *map, int type, int rank, const void *base, const uint64_t *dims, const uint64_t *strides,
                const uint32_t *box);
-size_t kv_attend_ws_bytes(int hd, int type);
+size_t kv_attend_ws_bytes(int hd);
 
 static size_t type_bytes(int type) { return type == CPG_T_F32 ? 4 : 2; }
 static bool type_ok(int type) { return type == CPG_T_F32 || type == CPG_T_F16 || type == CPG_T_BF16; }
@@ -415,7 +415,7 @@ extern "C" size_t cpg_kv_attend_workspace_bytes(const cpg_kv *kv, int n_heads) {
         set_error("cpg_kv_attend_workspace_bytes: bad argument");
         return 0;
     }
-    return kv_attend_ws_bytes(kv->hd, kv->v.type);
+    return kv_attend_ws_bytes(kv->hd);
 }
 
 extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads, const void *q,
@@ -436,7 +436,7 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     rc = rows_ok(fn, "q", q, q_stride, n_heads, kv->hd, type);
     if (!rc) rc = rows_ok(fn, "out", out, out_stride, n_heads, kv->hd, type);
     if (rc) return rc;
-    const size_t need = kv_attend_ws_bytes(kv->hd, kv->v.type);
+    const size_t need = kv_attend_ws_bytes(kv->hd);
     CPG_REQUIRE(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, "%s: workspace of %zu bytes at a 256-byte boundary needed, got %zu",
                 fn, need, ws ? ws_bytes : (size_t)0);
     return kv_attend_launch(kv->v, kv->maps, kv->hd, r, q, q_stride, out, out_stride, type, n_heads, scale, window, b->max_new, ws,

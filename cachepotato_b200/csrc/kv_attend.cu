@@ -832,6 +832,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 }
 
 int kv_attend_tc_launch(const AttendArgs &a, const CUtensorMap *maps, int hd, cudaStream_t s);
+int kv_attend_tcf_launch(const AttendArgs &a, const CUtensorMap *maps, int hd, cudaStream_t s);
 size_t kv_attend_tc_part_bytes(int hd);
 
 // Workspace: counters (of this kernel, then of the chunk kernel's), then the parts. The counters
@@ -840,10 +841,10 @@ constexpr size_t KD_COUNTERS = 3 * KV_MAX_GRID, KT_COUNTERS = 6 * KV_MAX_GRID;
 constexpr size_t KV_PARTS_AT = (KD_COUNTERS + KT_COUNTERS) * sizeof(int);
 static_assert(KV_PARTS_AT % 256 == 0, "parts start at a 256-byte boundary");
 
-size_t kv_attend_ws_bytes(int hd, int type) {
+size_t kv_attend_ws_bytes(int hd) {
     const size_t slot = (hd == 128 ? kd_slot<128>() : kd_slot<64>()) * sizeof(float);
     const size_t parts = 2 * (size_t)KV_MAX_GRID * slot;
-    return KV_PARTS_AT + (type == CPG_T_F32 ? parts : std::max(parts, kv_attend_tc_part_bytes(hd)));
+    return KV_PARTS_AT + std::max(parts, kv_attend_tc_part_bytes(hd));
 }
 
 template <typename TI, typename TC, int HD>
@@ -873,12 +874,12 @@ int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &
                  (float *)((uint8_t *)ws + KV_PARTS_AT), (int *)ws};
     const CUtensorMap *m = maps.m;
     // Rows of a sequence and cached head past one row tile of this file's kernel go to the chunk
-    // kernel: its 2 x 128 rows share each tile of K and V that is read.
+    // kernels: their 128 or 256 rows share each tile of K and V that is read.
     const int G = n_heads / c.KV;
     const long most = max_new > 0 ? std::min(max_new, b.T) : b.T;
-    if (type != CPG_T_F32 && G <= 128 && most * G > KD_ROWS) {
+    if (G <= 128 && most * G > KD_ROWS) {
         a.counters += KD_COUNTERS;
-        return kv_attend_tc_launch(a, m, hd, s);
+        return type == CPG_T_F32 ? kv_attend_tcf_launch(a, m, hd, s) : kv_attend_tc_launch(a, m, hd, s);
     }
     a.box = std::min(maps.box, KD_TILE);
     if (type == CPG_T_F32)

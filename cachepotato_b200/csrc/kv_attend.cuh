@@ -59,6 +59,7 @@ __device__ __forceinline__ long kv_div(long a, long b) {
 // Units 0..U-1 over NB blocks: block b has [start(b), start(b + 1)), the first U % NB one more.
 struct KvCut {
     long each, more;
+    KvCut() = default;
     __device__ __forceinline__ KvCut(long U, long NB) : each(kv_div(U, NB)), more(U - each * NB) {}
     __device__ __forceinline__ long start(long b) const { return b * each + min(b, more); }
     __device__ __forceinline__ int owner(long u) const {

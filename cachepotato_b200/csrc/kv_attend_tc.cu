@@ -32,77 +32,19 @@
 #include <algorithm>
 #include <atomic>
 
-#include "kv_attend.cuh"
+#include "kv_attend_tc.cuh"
 
 namespace cpg {
 
-constexpr int KT_TILE = 128, KT_ROWS = 128;               // positions and rows of an MMA tile
-constexpr int KT_THREADS = 384, KT_PRODUCER = 8, KT_MMA = 9, KT_FIXER = 10;
-constexpr int KT_FIXED = 2;                               // units an item's begin and end are worth (see KD_FIXED)
+constexpr int KT_TILE = 128;                              // positions of an MMA tile
 template <int HD> constexpr int kt_unit() { return KT_TILE * HD * 2; }
 template <int HD> constexpr int kt_units() { return HD == 128 ? 5 : 8; }
 template <int HD> constexpr int kt_smem() { return 1024 + 2 * KT_ROWS * HD * 2 + kt_units<HD>() * kt_unit<HD>(); }
-template <int HD> constexpr int kt_part() { return (2 + HD) * KT_ROWS; }       // floats of a row tile's part: m, l, o (four columns of a row together)
-static_assert(KT_ROWS == 128 && KT_TILE == 128, "tile shapes");
-
-// Sequence i in units. Pair p (of row tiles) holds tokens [p·Q, min(len, p·Q + Q)).
-struct KtSeq {
-    KvSeq s;
-    int pairs;
-    long head_units;                                      // of one cached head
-};
-// position tiles of pair p; with a window, from the first token's on
-__device__ __forceinline__ int kt_tiles(const AttendArgs &a, int Q, const KvSeq &s, int p) {
-    const int lo = a.window ? max(0, s.p0 + p * Q - a.window + 1) : 0;
-    return (s.p0 + min(s.len, p * Q + Q) - 1) / KT_TILE + 1 - lo / KT_TILE;
-}
-__device__ __forceinline__ KtSeq kt_seq(const AttendArgs &a, int Q, int i) {
-    KtSeq q;
-    q.s = kv_seq(a.b, a.c.P, i);
-    q.pairs = (q.s.len + Q - 1) / Q;
-    q.head_units = 0;
-    // a handful of instructions a pair; a closed form took longer than summing thousands of pairs
-    for (int p = 0; p < q.pairs; ++p) q.head_units += KT_FIXED + kt_tiles(a, Q, q.s, p);
-    return q;
-}
-
-// A place in the order of units: sequence, cached head, pair, position tile (kt from -KT_FIXED).
-struct KtCursor {
-    int seq, kh, pair, kt;
-    KvSeq s;
-    int pairs;
-    int lo_t, nt, hi;                                     // the item's position tiles; one past its last position
-    __device__ __forceinline__ int lo_of(const AttendArgs &a, int tok) const {
-        return a.window ? max(0, s.p0 + tok - a.window + 1) : 0;
-    }
-    __device__ __forceinline__ void item(const AttendArgs &a, int Q) {
-        hi = s.p0 + min(s.len, (pair + 1) * Q);
-        lo_t = lo_of(a, pair * Q) / KT_TILE;
-        nt = kt_tiles(a, Q, s, pair);
-    }
-    __device__ __forceinline__ void next_item(const AttendArgs &a, int Q) {
-        kt = -KT_FIXED;
-        if (++pair < pairs) {
-            item(a, Q);
-            return;
-        }
-        pair = 0;
-        if (++kh == a.c.KV) {
-            kh = 0;
-            do {
-                if (++seq >= a.b.n) return;
-                s = kv_seq(a.b, a.c.P, seq);
-            } while (s.len == 0);
-            pairs = (s.len + Q - 1) / Q;
-        }
-        item(a, Q);
-    }
-};
 
 // Row tile x of an item: tokens [t0, t1) of the sequence and the positions its rows see between them.
 struct KtRows {
     int t0, t1, lo, hi;
-    __device__ __forceinline__ KtRows(const AttendArgs &a, const KtCursor &c, int Q, int x) {
+    __device__ __forceinline__ KtRows(const AttendArgs &a, const KtCursor<KT_TILE> &c, int Q, int x) {
         t0 = c.pair * Q + x * (Q / 2);
         t1 = min(c.s.len, t0 + Q / 2);
         lo = c.lo_of(a, t0);
@@ -110,52 +52,6 @@ struct KtRows {
     }
     __device__ __forceinline__ bool sees(int j0) const { return j0 < hi && j0 + KT_TILE > lo; }
 };
-
-__device__ __forceinline__ bool kt_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    if (mbar_try_wait(smem_u32(bar), parity)) return true;
-    if (*abort_flag) return false;
-    if (mbar_wait(bar, parity)) return true;
-    *abort_flag = 1;
-    atomicOr(status, KV_TIMEOUT);
-    return false;
-}
-
-// The same for a whole warp, which goes on or leaves together.
-__device__ __forceinline__ bool kt_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    return __all_sync(0xffffffffu, kt_wait(bar, parity, abort_flag, status));
-}
-
-// Whether a V tile with `end` places up to the item's last position has more in that one's box.
-__device__ __forceinline__ bool kt_fix(const AttendArgs &a, int end) { return end < KT_TILE && end % a.box; }
-
-// Two f32 in one 64-bit register, worked on by one instruction (sm_100).
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-// Nothing that uses r may be moved before this point (the wait for the loads that fill it).
-__device__ __forceinline__ void settle16(uint32_t *r) {
-    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                      "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-}
-__device__ __forceinline__ void settle32(uint32_t *r) {
-    settle16(r);
-    settle16(r + 16);
-}
 
 template <bool HALF, int HD>
 __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_constant__ AttendArgs a,
@@ -169,8 +65,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, asked[NU], fixed[NU], s_full[2], p_full[2], o_full[2], drain;
-    __shared__ long s_scan[KT_THREADS / 32], s_cut[2], s_off;
-    __shared__ KtCursor s_cur;
+    __shared__ KtShared<KT_TILE> sh;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_last[2], s_ask[NU][3];     // a V tile to clear: ring slot, its fill's parity, first place
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -199,96 +94,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- this block's range of units, and the item it starts in
-    const int n = a.b.n, blk = blockIdx.x;
-    long U = 0, before = 0, u0 = 0, u1 = 0;
-    int NB = 0;
-    KvCut cut(0, 1);
-    auto range = [&](long total) {                        // false: nothing for this block
-        U = total;
-        NB = (int)min((long)gridDim.x, U);
-        if (blk >= NB) return false;
-        cut = KvCut(U, NB);
-        u0 = cut.start(blk);
-        u1 = cut.start(blk + 1);
-        return true;
-    };
-    if (n > KT_THREADS) {                                 // more sequences than threads: their sum first
-        long sum = 0;
-        for (int i = tid; i < n; i += KT_THREADS) sum += kt_seq(a, Q, i).head_units * a.c.KV;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s_scan[warp] = sum;
-        __syncthreads();
-        sum = 0;
-        for (int w = 0; w < KT_THREADS / 32; ++w) sum += s_scan[w];
-        if (!range(sum)) return;
-        __syncthreads();
-    }
-    for (int c0 = 0; c0 < n; c0 += KT_THREADS) {          // THREADS sequences at a time
-        KtSeq mine{};
-        if (c0 + tid < n) {
-            mine = kt_seq(a, Q, c0 + tid);
-            if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
-        }
-        const long x = mine.head_units * a.c.KV;
-        long inc = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 31) s_scan[warp] = inc;
-        __syncthreads();
-        long base = before, all = 0;
-        for (int w = 0; w < KT_THREADS / 32; ++w) {
-            if (w < warp) base += s_scan[w];
-            all += s_scan[w];
-        }
-        if (n <= KT_THREADS && !range(all)) return;
-        const long at = u0 - (base + inc - x);
-        if (at >= 0 && at < x) {
-            KtCursor c;
-            c.seq = c0 + tid;
-            c.s = mine.s;
-            c.pairs = mine.pairs;
-            c.kh = (int)kv_div(at, mine.head_units);
-            s_off = at - c.kh * mine.head_units;
-            s_cur = c;
-        }
-        before += all;
-        __syncthreads();
-        if (u0 < before) break;
-    }
-    if (u0 >= u1) return;                                 // no sequences at all
-    if (tid == 0) {
-        s_cut[0] = cut.each;
-        s_cut[1] = cut.more;
-    }
-    if (warp == 0) {                                      // the pair that holds unit s_off, 32 pairs at a time
-        KtCursor c = s_cur;
-        long off = s_off;
-        for (int p0 = 0; p0 < c.pairs; p0 += 32) {
-            const int p = p0 + lane, mine = p < c.pairs ? KT_FIXED + kt_tiles(a, Q, c.s, p) : 0;
-            int inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            const int all = __shfl_sync(0xffffffffu, inc, 31);
-            if (off < all) {
-                if (off >= inc - mine && off < inc) {
-                    c.pair = p;
-                    c.kt = (int)off - (inc - mine) - KT_FIXED;
-                    c.item(a, Q);
-                    s_cur = c;
-                }
-                break;
-            }
-            off -= all;
-        }
-    }
+    long u0, u1;                                          // this block's range of units
+    if (!kt_begin<KT_TILE>(a, Q, sh, u0, u1)) return;
     if (warp == KT_MMA) {                                 // all of TMEM
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -300,7 +107,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     volatile int *const abort_flag = &s_abort;
     int *const status = a.c.status;
     const uint32_t sq = smem_u32(smem), ring = sq + 2 * QT;
-    KtCursor cur = s_cur;
+    KtCursor<KT_TILE> cur = sh.cur;
     // skips an item's fixed share: false if nothing of the item itself is this block's
     auto begin = [&](long &u) {
         if (cur.kt < 0) {
@@ -350,7 +157,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         if (lane < boxes)
                             tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
                                         lane % PARTS * 64, place, cur.kh, page, &full[slot]);
-                        if (half && kt_fix(a, cur.hi - j0)) {
+                        if (half && kt_fix(a, KT_TILE, cur.hi - j0)) {
                             if (lane == 0) {
                                 s_ask[asks % NU][0] = slot;
                                 s_ask[asks % NU][1] = turn & 1;
@@ -427,7 +234,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         const bool more = i + 1 < n_here;
                         const bool n0 = more && r0.sees(j0 + KT_TILE), n1 = more && r1.sees(j0 + KT_TILE);
                         ok = wait(&full[vs], vp) && (!more || wait(&full[ks], kp));
-                        if (ok && kt_fix(a, cur.hi - j0)) {
+                        if (ok && kt_fix(a, KT_TILE, cur.hi - j0)) {
                             ok = wait(&fixed[vs], fp >> vs & 1u);
                             fp ^= 1u << vs;
                         }
@@ -475,7 +282,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
             for (long u = u0; u < u1;) {
                 if (!begin(u)) break;
                 const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                if (kt_fix(a, cur.hi - (cur.lo_t + cur.kt + n_here - 1) * KT_TILE)) {
+                if (kt_fix(a, KT_TILE, cur.hi - (cur.lo_t + cur.kt + n_here - 1) * KT_TILE)) {
                     const int at = asks % NU;
                     if (!kt_wait_warp(&asked[at], (uint32_t)(asks / NU) & 1u, abort_flag, status)) break;
                     const int slot = s_ask[at][0], end = s_ask[at][2];
@@ -645,10 +452,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
             // ---- the item, or this block's part of it, is done: its tiles are units [ua, ue), blocks b0..b1
             const long ua = u - cur.kt, ue = ua + cur.nt;
             u += n_here;
-            KvCut shares(0, 1);
-            shares.each = s_cut[0];
-            shares.more = s_cut[1];
-            const int b0 = shares.owner(ua), b1 = shares.owner(ue - 1);
+            const int b0 = sh.cut.owner(ua), b1 = sh.cut.owner(ue - 1);
             const size_t cell = (size_t)(cur.s.r0 + rt.t0 + tok);
             uint16_t *const dst = (uint16_t *)a.out + cell * a.out_stride + (size_t)(cur.kh * G + g) * HD;
             // 16 columns from c of the row, times f, to out
@@ -686,96 +490,23 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     write16(c, v, inv);
                 }
             } else {
-                const int np = b1 - b0 + 1, pi = blk - b0;
+                const int np = b1 - b0 + 1, pi = (int)blockIdx.x - b0;
                 int gs = np;
                 if (np > 4)
                     for (gs = 2; gs * gs < np;) ++gs;
                 const int ng = (np + gs - 1) / gs, gi = pi / gs, n_in = min(gs, np - gi * gs);
-                auto slot_of = [&](int k) { return k == 0 ? 2 * b0 + 1 : 2 * (b0 + k); };
-                auto part = [&](int k) { return a.part + ((size_t)slot_of(k) * 2 + x) * kt_part<HD>(); };
-                auto put16 = [&](float *to, int c, const float *v) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        __stcg(reinterpret_cast<float4 *>(to + 2 * KT_ROWS) + (c / 4 + e) * KT_ROWS + row,
-                               make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
-                };
-                float *to = part(pi);
+                const KtParts<HD> parts{a.part, x, row, b0};
+                float *to = parts.at(pi);
                 __stcg(to + row, m);
                 __stcg(to + KT_ROWS + row, l);
 #pragma unroll 2
                 for (int c = 0; c < HD; c += 16) {
                     float v[16];
                     load16(c, v);
-                    put16(to, c, v);
+                    parts.put16(to, c, v);
                 }
-                // parts first, first + step, ... (count of them), joined by the last of their blocks:
-                // into the first one's place, or (last) into out
-                auto join = [&](int *counter, int firstp, int step, int count, bool last) -> bool {
-                    named_bar_sync(1 + x, 128);
-                    if (row == 0) {
-                        __threadfence();
-                        const int mine = atomicAdd(counter, 1) == count - 1;
-                        if (mine) *counter = 0;           // ready for the next call
-                        __threadfence();
-                        s_last[x] = mine;
-                    }
-                    named_bar_sync(1 + x, 128);
-                    const bool mine = s_last[x] != 0;
-                    named_bar_sync(1 + x, 128);
-                    if (!mine) return false;
-                    float M = -INFINITY, L = 0.0f;
-#pragma unroll 4
-                    for (int k = 0; k < count; ++k) M = fmaxf(M, __ldcg(part(firstp + k * step) + row));
-                    const float bs = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-                    for (int k = 0; k < count; ++k)
-                        L = fmaf(ex2(__ldcg(part(firstp + k * step) + row) - bs), __ldcg(part(firstp + k * step) + KT_ROWS + row), L);
-                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                    float *put = part(firstp);
-#pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        float v[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
-                        for (int k = 0; k < count; k += 2) {              // two parts' columns in flight
-                            float4 y[2][8];
-                            float w[2];
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const float *src = part(firstp + min(k + z, count - 1) * step);
-                                w[z] = __ldcg(src + row);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    y[z][e] = __ldcg(reinterpret_cast<const float4 *>(src + 2 * KT_ROWS) + (c / 4 + e) * KT_ROWS + row);
-                            }
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const float f = k + z < count ? ex2(w[z] - bs) : 0.0f;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    v[4 * e] = fmaf(f, y[z][e].x, v[4 * e]);
-                                    v[4 * e + 1] = fmaf(f, y[z][e].y, v[4 * e + 1]);
-                                    v[4 * e + 2] = fmaf(f, y[z][e].z, v[4 * e + 2]);
-                                    v[4 * e + 3] = fmaf(f, y[z][e].w, v[4 * e + 3]);
-                                }
-                            }
-                        }
-                        if (last) {
-                            write16(c, v, inv);
-                            write16(c + 16, v + 16, inv);
-                        } else {
-                            put16(put, c, v);
-                            put16(put, c + 16, v + 16);
-                        }
-                    }
-                    if (!last) {
-                        __stcg(put + row, M);
-                        __stcg(put + KT_ROWS + row, L);
-                    }
-                    return true;
-                };
-                if (join(a.counters + slot_of(gi * gs) * 2 + x, gi * gs, 1, n_in, ng == 1) && ng > 1)
-                    join(a.counters + 4 * KV_MAX_GRID + b0 * 2 + x, 0, gs, ng, true);
+                if (parts.join(a.counters + parts.slot_of(gi * gs) * 2 + x, &s_last[x], gi * gs, 1, n_in, ng == 1, write16) && ng > 1)
+                    parts.join(a.counters + 4 * KV_MAX_GRID + b0 * 2 + x, &s_last[x], 0, gs, ng, true, write16);
             }
             tc_fence_before();
             if (u < u1) cur.next_item(a, Q);
