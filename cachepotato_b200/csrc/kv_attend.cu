@@ -873,11 +873,14 @@ int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &
     AttendArgs a{b, c, q, out, q_stride, out_stride, n_heads, scale * 1.4426950408889634f, window, maps.box,
                  (float *)((uint8_t *)ws + KV_PARTS_AT), (int *)ws};
     const CUtensorMap *m = maps.m;
-    // Rows of a sequence and cached head past one row tile of this file's kernel go to the chunk
-    // kernels: their 128 or 256 rows share each tile of K and V that is read.
+    // Past two row tiles of this file's kernel per sequence and cached head the chunk kernels take over:
+    // their 128 or 256 rows share each tile of K and V that is read, but beginning and joining cost
+    // them more. Measured (us, few / chunk, 4 cached heads of 128): 32 rows of one sequence over 4096
+    // positions 17 / 37 in bf16 and 22 / 36 in f32, of 64 sequences over 1000 62 / 56 and 134 / 141;
+    // 64 rows 19 / 36 and 29 / 35, 107 / 54 and 247 / 141.
     const int G = n_heads / c.KV;
     const long most = max_new > 0 ? std::min(max_new, b.T) : b.T;
-    if (G <= 128 && most * G > KD_ROWS) {
+    if (G <= 128 && most * G > 2 * KD_ROWS) {
         a.counters += KD_COUNTERS;
         return type == CPG_T_F32 ? kv_attend_tcf_launch(a, m, hd, s) : kv_attend_tc_launch(a, m, hd, s);
     }

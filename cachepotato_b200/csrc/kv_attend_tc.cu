@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                 if (np > 4)
                     for (gs = 2; gs * gs < np;) ++gs;
                 const int ng = (np + gs - 1) / gs, gi = pi / gs, n_in = min(gs, np - gi * gs);
-                const KtParts<HD> parts{a.part, x, row, b0};
+                const KtParts<HD> parts{a.part, x, row, b0, live};
                 float *to = parts.at(pi);
                 __stcg(to + row, m);
                 __stcg(to + KT_ROWS + row, l);

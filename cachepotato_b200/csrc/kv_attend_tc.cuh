@@ -223,9 +223,11 @@ template <int HD>
 struct KtParts {
     float *base;
     int x, row, b0;
+    bool live;                                            // rows that hold nothing are neither left nor read
     __device__ __forceinline__ int slot_of(int k) const { return k == 0 ? 2 * b0 + 1 : 2 * (b0 + k); }
     __device__ __forceinline__ float *at(int k) const { return base + ((size_t)slot_of(k) * 2 + x) * kt_part<HD>(); }
     __device__ __forceinline__ void put16(float *to, int c, const float *v) const {
+        if (!live) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             __stcg(reinterpret_cast<float4 *>(to + 2 * KT_ROWS) + (c / 4 + e) * KT_ROWS + row,
@@ -247,6 +249,7 @@ struct KtParts {
         const bool mine = *s_last != 0;
         named_bar_sync(1 + x, 128);
         if (!mine) return false;
+        if (!live) return true;
         float M = -INFINITY, L = 0.0f;
 #pragma unroll 4
         for (int k = 0; k < count; ++k) M = fmaxf(M, __ldcg(at(first + k * step) + row));

@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                 if (np > 4)
                     for (gs = 2; gs * gs < np;) ++gs;
                 const int ng = (np + gs - 1) / gs, gi = pi / gs, n_in = min(gs, np - gi * gs);
-                const KtParts<HD> parts{a.part, 0, row, b0};
+                const KtParts<HD> parts{a.part, 0, row, b0, live};
                 float *to = parts.at(pi);
                 __stcg(to + row, m);
                 __stcg(to + KT_ROWS + row, l);
