@@ -280,57 +280,58 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     volatile int *const abort_flag = &s_abort;
 
     if (warp == KD_WARPS) {
-        // ---- producer: lane b loads box b of every unit (box = position group · PARTS + column)
-        const int groups = KD_TILE / a.box;
+        // ---- producer: lane b loads box b of every unit (box = position group · PARTS + column, at
+        // most 8 groups of 4)
+        const int boxes = KD_TILE / a.box * PARTS;
         const uint32_t ring = smem_u32(smem);
         int slot = 0, turn = 0;
         bool stop = false;
-        for (long u = u0; u < u1; ++u) {
+        for (long u = u0; u < u1 && !stop;) {
             if (cur.kt < 0) {                             // nothing to load
-                ++cur.kt;
-                continue;
+                u -= cur.kt;
+                cur.kt = 0;
+                if (u >= u1) break;
             }
-            const int j0 = (cur.r.lo_t + cur.kt) * KD_TILE;
-            const int boxes = groups * PARTS;
-            int page[2], place[2];                        // boxes lane, lane + 32 (at most 8 groups of 4)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int bx = lane + 32 * x, j = j0 + bx / PARTS * a.box;
-                page[x] = a.c.n_pages;                    // outside the pool: zeros
-                place[x] = 0;
-                if (bx < boxes && j < cur.r.hi && j + a.box > cur.r.lo) {
+            const int n_here = (int)min((long)(cur.r.nt - cur.kt), u1 - u);
+            // page and place of this lane's box of tile i; the next tile's is asked for ahead
+            auto find = [&](int i, int &page, int &place) {
+                const int j = (cur.r.lo_t + cur.kt + i) * KD_TILE + lane / PARTS * a.box;
+                place = -1;                               // nothing of it is seen
+                if (lane < boxes && i < n_here && j < cur.r.hi && j + a.box > cur.r.lo) {
                     const int pg = j / a.c.P;
-                    const int id = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
-                    if (id >= 0 && id < a.c.n_pages) page[x] = id;
-                    else atomicOr(a.c.status, KV_BAD_PAGE);
-                    place[x] = j - pg * a.c.P;
+                    page = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
+                    place = j - pg * a.c.P;
+                }
+            };
+            int next_page = 0, next_place;
+            find(0, next_page, next_place);
+            for (int i = 0; i < n_here && !stop; ++i) {
+                const bool inside = next_place >= 0 && next_page >= 0 && next_page < a.c.n_pages;
+                if (next_place >= 0 && !inside) atomicOr(a.c.status, KV_BAD_PAGE);
+                const int page = inside ? next_page : a.c.n_pages, place = max(next_place, 0);   // outside the pool: zeros
+                find(i + 1, next_page, next_place);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {    // K, then V
+                    const bool ok = !turn || *abort_flag || mbar_wait(&empty[slot], (uint32_t)(turn - 1) & 1u);
+                    if (!ok) {
+                        *abort_flag = 1;
+                        atomicOr(a.c.status, KV_TIMEOUT);
+                    }
+                    stop = __any_sync(0xffffffffu, !ok || *abort_flag);
+                    if (stop) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
+                    __syncwarp();
+                    if (lane < boxes)
+                        tma_load_4d(ring + slot * UNIT + lane % PARTS * (KD_TILE * 128) + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
+                                    lane % PARTS * (128 / ES), place, cur.kh, page, &full[slot]);
+                    if (++slot == NU) {
+                        slot = 0;
+                        ++turn;
+                    }
                 }
             }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {        // K, then V
-                const bool ok = !turn || *abort_flag || mbar_wait(&empty[slot], (uint32_t)(turn - 1) & 1u);
-                if (!ok) {
-                    *abort_flag = 1;
-                    atomicOr(a.c.status, KV_TIMEOUT);
-                }
-                stop = __any_sync(0xffffffffu, !ok || *abort_flag);
-                if (stop) break;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
-                __syncwarp();
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int bx = lane + 32 * x, part = bx % PARTS;
-                    if (bx < boxes)
-                        tma_load_4d(ring + slot * UNIT + part * (KD_TILE * 128) + bx / PARTS * a.box * 128, half ? &tm_v : &tm_k,
-                                    part * (128 / ES), place[x], cur.kh, page[x], &full[slot]);
-                }
-                if (++slot == NU) {
-                    slot = 0;
-                    ++turn;
-                }
-            }
-            if (stop) break;
-            if (++cur.kt == cur.r.nt && u + 1 < u1) cur.next_item(a, G);
+            u += n_here;
+            if (u < u1 && !stop) cur.next_item(a, G);
         }
         if (stop) {                                       // copies in flight land before the block may end
             for (int i = 0; i < NU; ++i) {

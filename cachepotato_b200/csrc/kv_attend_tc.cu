@@ -6,26 +6,23 @@
 // cycles of both q·k and p·v at HD = 128, and 1024 cycles for its 16384 exponentials.
 //   work    A sequence's rows are (token, head) pairs per cached head. An item is (sequence, cached
 //           head, pair of row tiles): two tiles of 128/G tokens x G heads, M = 128 rows each, that
-//           share every K and V tile read from L2. Its units are tiles of 128 positions; the units of
+//           share every K and V tile read from L2. Its units are tiles of 64 positions; the units of
 //           all items are cut into equal ranges, one per SM (as in kv_attend.cu: causal items of all
 //           lengths, one long one or hundreds of short ones fill the GPU the same way).
 //   block   warps 0-3, 4-7  softmax of row tile 0 and 1, one thread per row: S out of TMEM, running
 //                           maximum and sum, P (16-bit) back over S; at an item's end O out of TMEM.
 //                           O is rescaled in place, and only when a row's maximum has grown by more
 //                           than 2^8 since the last time: the scale cancels in O / l, and f32 and the
-//                           cache's types hold weights up to 2^8 as well as up to 1. So a tile's
-//                           weights are taken with the maximum at hand, in one pass over S, and only
-//                           if it proves too small are they taken again. (An item's first tile is
-//                           gone over for the maximum first.)
-//           warp 8          producer: q tiles and the ring of K and V tiles, tensor TMA
-//           warp 9          tcgen05.mma: S = q·K^T (both operands in shared memory), O += P·V (P from
-//                           TMEM). While one row tile is in its softmax the other's products run.
-//           warp 10         clears the places of an item's last V tile that lie in its last page behind
-//                           the last position (they may hold anything, and 0 · NaN is NaN)
-//           TMEM: S0 S1 | O0 O1, 128 columns each; P lies over its S.
-//   order   The tensor core runs what one thread issues in order, so q·k of the next tile may be
-//           issued behind the p·v that still reads P from the same columns, and a finished q·k says
-//           that the p·v before it has finished: between then and its own P the softmax owns O.
+//                           cache's types hold weights up to 2^8 as well as up to 1.
+//           warps 8, 10     producers of q and the K tiles, and of the V tiles: tensor TMA into a ring
+//           warps 9, 11     tcgen05.mma of row tile 0 and 1: S = q·K^T (both operands in shared memory),
+//                           O += P·V (P from TMEM). One thread for both row tiles was the limit: its
+//                           waits for tiles that are there take 100 to 250 cycles each.
+//           TMEM: two S of 64 columns for each row tile | O0 O1 of 128; P lies over its S.
+//   order   With two S a row tile's next q·k runs while the softmax works on this one, so neither waits
+//           for the other unless it is the slower (one S of 128 columns, q·k behind p·v: 3900 cycles
+//           for two row tiles and 128 positions, of which the tensor core worked half). The tensor core
+//           runs what one thread issues in order, so q·k may overwrite P of the tile before last.
 //   join    Parts of an item that several blocks share, as in kv_attend.cu.
 #include <math.h>
 
@@ -36,15 +33,15 @@
 
 namespace cpg {
 
-constexpr int KT_TILE = 128;                              // positions of an MMA tile
+constexpr int KT_TILE = 64, KT_FIXED = 4;                 // positions of an MMA tile; units an item's begin and end are worth
 template <int HD> constexpr int kt_unit() { return KT_TILE * HD * 2; }
-template <int HD> constexpr int kt_units() { return HD == 128 ? 5 : 8; }
+template <int HD> constexpr int kt_units() { return HD == 128 ? 10 : 16; }
 template <int HD> constexpr int kt_smem() { return 1024 + 2 * KT_ROWS * HD * 2 + kt_units<HD>() * kt_unit<HD>(); }
 
 // Row tile x of an item: tokens [t0, t1) of the sequence and the positions its rows see between them.
 struct KtRows {
     int t0, t1, lo, hi;
-    __device__ __forceinline__ KtRows(const AttendArgs &a, const KtCursor<KT_TILE> &c, int Q, int x) {
+    __device__ __forceinline__ KtRows(const AttendArgs &a, const KtCursor<KT_TILE, KT_FIXED> &c, int Q, int x) {
         t0 = c.pair * Q + x * (Q / 2);
         t1 = min(c.s.len, t0 + Q / 2);
         lo = c.lo_of(a, t0);
@@ -58,33 +55,37 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                                                                const __grid_constant__ CUtensorMap tm_q,
                                                                const __grid_constant__ CUtensorMap tm_k,
                                                                const __grid_constant__ CUtensorMap tm_v) {
-    constexpr int PARTS = HD / 64, COL = KT_TILE * 128;   // 128-byte columns of a tile, bytes of one
+    constexpr int PARTS = HD / 64;                        // 128-byte columns of a row
+    constexpr int COL = KT_TILE * 128, QCOL = KT_ROWS * 128;   // bytes of one in a K or V tile, in a row tile
     constexpr int UNIT = kt_unit<HD>(), NU = kt_units<HD>(), QT = KT_ROWS * HD * 2;
     constexpr uint32_t FMT = HALF ? 0u : UMMA_BF16;
     constexpr uint32_t ID_QK = umma_idesc_f16(128, KT_TILE) | FMT, ID_PV = umma_idesc_f16(128, HD) | FMT | UMMA_B_MN;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, asked[NU], fixed[NU], s_full[2], p_full[2], o_full[2], drain;
-    __shared__ KtShared<KT_TILE> sh;
+    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, fixed[NU], s_full[2][2], p_full[2][2], o_done[2],
+        drain[2];
+    __shared__ KtShared<KT_TILE, KT_FIXED> sh;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_last[2], s_ask[NU][3];     // a V tile to clear: ring slot, its fill's parity, first place
+    __shared__ int s_abort, s_last[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = a.H / a.c.KV, TT = KT_ROWS / G, Q = 2 * TT;             // tokens of a row tile, of a pair
     if (tid == 0) {
         for (int i = 0; i < NU; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-            mbar_init(&asked[i], 1);
+            mbar_init(&empty[i], 2);
             mbar_init(&fixed[i], 1);
         }
         mbar_init(&q_full, 1);
-        mbar_init(&q_empty, 1);
+        mbar_init(&q_empty, 2);
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[x], 4);
-            mbar_init(&o_full[x], 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&s_full[x][b], 1);
+                mbar_init(&p_full[x][b], 4);
+            }
+            mbar_init(&o_done[x], 1);
         }
-        mbar_init(&drain, 1);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
         fence_mbar_init();
         s_abort = 0;
         prefetch_map(&tm_q);
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     pdl_launch_dependents();
 
     long u0, u1;                                          // this block's range of units
-    if (!kt_begin<KT_TILE>(a, Q, sh, u0, u1)) return;
+    if (!kt_begin<KT_TILE, KT_FIXED>(a, Q, sh, u0, u1)) return;
     if (warp == KT_MMA) {                                 // all of TMEM
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     volatile int *const abort_flag = &s_abort;
     int *const status = a.c.status;
     const uint32_t sq = smem_u32(smem), ring = sq + 2 * QT;
-    KtCursor<KT_TILE> cur = sh.cur;
+    KtCursor<KT_TILE, KT_FIXED> cur = sh.cur;
     // skips an item's fixed share: false if nothing of the item itself is this block's
     auto begin = [&](long &u) {
         if (cur.kt < 0) {
@@ -118,76 +119,95 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     };
 
     if (warp >= 8) {
-        if (warp == KT_PRODUCER) {
-            // ---------------- producer: lane b loads box b of every unit
-            const int groups = KT_TILE / a.box, boxes = groups * PARTS;
-            int slot = 0, turn = 0, items = 0, asks = 0;
+        if (warp == KT_LOAD_K || warp == KT_LOAD_V) {
+            // ---------------- producers: K tiles (and q) in the ring's even slots, V tiles in the odd
+            // ones. Lane b loads box b of a tile: issuing small boxes (16 positions: 2 KB) takes a warp
+            // some 50 cycles each, so one warp for both was the limit.
+            const bool is_v = warp == KT_LOAD_V;
+            const CUtensorMap *const map = is_v ? &tm_v : &tm_k;
+            const int boxes = KT_TILE / a.box * PARTS;
+            int slot = is_v, turn = 0, items = 0;
             bool ok = true;
             for (long u = u0; u < u1 && ok;) {
                 if (!begin(u)) break;
-                if (items && !kt_wait_warp(&q_empty, (uint32_t)(items - 1) & 1u, abort_flag, status)) break;
                 const KtRows r0(a, cur, Q, 0), r1(a, cur, Q, 1);
-                const bool two = r1.t1 > r1.t0;
-                if (lane == 0) mbar_arrive_expect_tx(&q_full, (two ? 2u : 1u) * (uint32_t)(TT * G * 128 * PARTS));
-                __syncwarp();
-                if (lane < 2 * PARTS && (two || lane < PARTS)) {
-                    const int x = lane / PARTS, part = lane % PARTS;
-                    tma_load_3d(sq + x * QT + part * COL, &tm_q, part * 64, cur.kh * G, cur.s.r0 + (x ? r1.t0 : r0.t0), &q_full);
+                if (!is_v) {
+                    ok = !items || kt_wait_warp(&q_empty, (uint32_t)(items - 1) & 1u, abort_flag, status);
+                    if (!ok) break;
+                    const bool two = r1.t1 > r1.t0;
+                    if (lane == 0) mbar_arrive_expect_tx(&q_full, (two ? 2u : 1u) * (uint32_t)(TT * G * 128 * PARTS));
+                    __syncwarp();
+                    if (lane < 2 * PARTS && (two || lane < PARTS)) {
+                        const int x = lane / PARTS, part = lane % PARTS;
+                        tma_load_3d(sq + x * QT + part * QCOL, &tm_q, part * 64, cur.kh * G, cur.s.r0 + (x ? r1.t0 : r0.t0), &q_full);
+                    }
+                    ++items;
                 }
-                ++items;
                 const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
                 const int lo = r0.lo;
-                for (int i = 0; i < n_here; ++i) {
-                    const int j0 = (cur.lo_t + cur.kt + i) * KT_TILE;
-                    int page = a.c.n_pages, place = 0;    // outside the pool: zeros
-                    const int j = j0 + lane / PARTS * a.box;
-                    if (lane < boxes && j < cur.hi && j + a.box > lo) {
+                // page and place of this lane's box of tile i; the next tile's is asked for ahead
+                auto find = [&](int i, int &page, int &place) {
+                    const int j = (cur.lo_t + cur.kt + i) * KT_TILE + lane / PARTS * a.box;
+                    place = -1;                           // nothing of it is seen
+                    if (lane < boxes && i < n_here && j < cur.hi && j + a.box > lo) {
                         const int pg = j / a.c.P;
-                        const int id = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
-                        if (id >= 0 && id < a.c.n_pages) page = id;
-                        else atomicOr(status, KV_BAD_PAGE);
+                        page = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
                         place = j - pg * a.c.P;
                     }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {                // K, then V
-                        ok = !turn || kt_wait_warp(&empty[slot], (uint32_t)(turn - 1) & 1u, abort_flag, status);
-                        if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
-                        __syncwarp();
-                        if (lane < boxes)
-                            tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
-                                        lane % PARTS * 64, place, cur.kh, page, &full[slot]);
-                        if (half && kt_fix(a, KT_TILE, cur.hi - j0)) {
-                            if (lane == 0) {
-                                s_ask[asks % NU][0] = slot;
-                                s_ask[asks % NU][1] = turn & 1;
-                                s_ask[asks % NU][2] = cur.hi - j0;
-                                mbar_arrive(&asked[asks % NU]);
-                            }
-                            ++asks;
-                        }
-                        if (++slot == NU) {
-                            slot = 0;
-                            ++turn;
-                        }
-                    }
+                };
+                int next_page = 0, next_place;
+                find(0, next_page, next_place);
+                for (int i = 0; i < n_here; ++i) {
+                    const bool inside = next_place >= 0 && next_page >= 0 && next_page < a.c.n_pages;
+                    if (next_place >= 0 && !inside) atomicOr(status, KV_BAD_PAGE);
+                    const int page = inside ? next_page : a.c.n_pages, place = max(next_place, 0);   // outside the pool: zeros
+                    find(i + 1, next_page, next_place);
+                    ok = !turn || kt_wait_warp(&empty[slot], (uint32_t)(turn - 1) & 1u, abort_flag, status);
                     if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
+                    __syncwarp();
+                    if (lane < boxes)
+                        tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, map, lane % PARTS * 64,
+                                    place, cur.kh, page, &full[slot]);
+                    // places of the last V tile behind the last position, in its box, may hold anything:
+                    // they are cleared before anyone reads the tile
+                    const int end = cur.hi - (cur.lo_t + cur.kt + i) * KT_TILE;
+                    if (is_v && kt_fix(a, KT_TILE, end)) {
+                        ok = kt_wait_warp(&full[slot], (uint32_t)turn & 1u, abort_flag, status);
+                        if (!ok) break;
+                        const int rows_z = (end + a.box - 1) / a.box * a.box - end;
+                        for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
+                            const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
+                            *reinterpret_cast<uint4 *>(smem + 2 * QT + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&fixed[slot]);
+                    }
+                    slot += 2;
+                    if (slot >= NU) {
+                        slot -= NU;
+                        ++turn;
+                    }
                 }
+                if (!ok) break;
                 u += n_here;
                 if (u < u1) cur.next_item(a, Q);
             }
-            if (*abort_flag) {                            // copies in flight land before the block may end
-                for (int i = 0; i < NU; ++i) {
+            if (!ok) {                                    // copies in flight land before the block may end
+                for (int i = is_v; i < NU; i += 2) {
                     const int fills = turn + (i < slot);
                     if (fills) mbar_wait(&full[i], (uint32_t)(fills - 1) & 1u);
                 }
                 if (items) mbar_wait(&q_full, (uint32_t)(items - 1) & 1u);
             }
-        } else if (warp == KT_MMA) {
-            // ---------------- tensor core: one elected lane waits and issues
+        } else {
+            // ---------------- tensor core, row tile x: one elected lane waits and issues
+            const int x = warp == KT_MMA ? 0 : 1;
             if (elect_one()) {
                 int ks = 0, vs = 1;                       // ring slots of the next K and V
-                uint32_t kp = 0, vp = 0, pp0 = 0, pp1 = 0, qp = 0, fp = 0;               // fp: a bit per slot
+                uint32_t kp = 0, vp = 0, pp = 0, qp = 0, fp = 0;           // parities; pp, fp: a bit per P, per slot
+                uint32_t qb = 0, pb = 0;                  // the S of the next q·k, the P of the next p·v
                 auto step2 = [&](int &s, uint32_t &ph) {
                     s += 2;
                     if (s >= NU) {
@@ -196,110 +216,69 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     }
                 };
                 auto wait = [&](uint64_t *bar, uint32_t parity) { return kt_wait(bar, parity, abort_flag, status); };
+                const uint64_t dq = umma_desc_sw128(sq + x * QT);
+                const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
+                // S = q · K^T from the next K (if the row tile sees it), which is then let go
+                auto qk = [&](bool sees, bool last) {
+                    if (!wait(&full[ks], kp)) return false;
+                    tc_fence_after();
+                    if (sees) {
+                        const uint64_t dk = umma_desc_sw128(ring + ks * UNIT);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k)
+                            umma_f16(tS + qb * KT_TILE, dq + ((k / 4 * QCOL + k % 4 * 32) >> 4), dk + ((k / 4 * COL + k % 4 * 32) >> 4),
+                                     ID_QK, k ? 1u : 0u);
+                        umma_commit(&s_full[x][qb]);
+                        qb ^= 1;
+                    }
+                    umma_commit(&empty[ks]);
+                    if (last) umma_commit(&q_empty);
+                    step2(ks, kp);
+                    return true;
+                };
                 bool ok = true;
                 for (long u = u0; u < u1 && ok;) {
                     if (!begin(u)) break;
-                    const KtRows r0(a, cur, Q, 0), r1(a, cur, Q, 1);
+                    const KtRows rt(a, cur, Q, x);
                     const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
                     const int first = (cur.lo_t + cur.kt) * KT_TILE;
                     if (!wait(&q_full, qp)) break;
                     qp ^= 1;
-                    bool begun0 = false, begun1 = false;
-                    // S_x = q_x · K^T from ring slot ks, O_x += P_x · V from slot vs; x = 0, 1
-                    auto qk = [&](int x) {
-                        const uint64_t dq = umma_desc_sw128(sq + x * QT), dk = umma_desc_sw128(ring + ks * UNIT);
-#pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) {
-                            const uint32_t at = (k / 4 * COL + k % 4 * 32) >> 4;       // of the descriptor's start
-                            umma_f16(tmem + x * 128, dq + at, dk + at, ID_QK, k ? 1u : 0u);
-                        }
-                        umma_commit(&s_full[x]);
-                    };
-                    auto pv = [&](int x, bool begun) {
-                        const uint64_t dv = umma_desc_sw128_mn(ring + vs * UNIT, COL);
-#pragma unroll
-                        for (int k = 0; k < KT_TILE / 16; ++k)
-                            umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, dv + (k * 2048 >> 4), ID_PV, begun || k ? 1u : 0u);
-                    };
-                    if (!wait(&full[ks], kp)) break;
-                    tc_fence_after();
-                    bool s0 = r0.sees(first), s1 = r1.sees(first);         // whether the row tiles see this unit
-                    if (s0) qk(0);
-                    if (s1) qk(1);
-                    umma_commit(&empty[ks]);
-                    if (n_here == 1) umma_commit(&q_empty);
-                    step2(ks, kp);
-                    for (int i = 0; i < n_here; ++i) {
+                    bool begun = false;
+                    ok = qk(rt.sees(first), n_here == 1);
+                    for (int i = 0; i < n_here && ok; ++i) {
                         const int j0 = first + i * KT_TILE;
-                        const bool more = i + 1 < n_here;
-                        const bool n0 = more && r0.sees(j0 + KT_TILE), n1 = more && r1.sees(j0 + KT_TILE);
-                        ok = wait(&full[vs], vp) && (!more || wait(&full[ks], kp));
-                        if (ok && kt_fix(a, KT_TILE, cur.hi - j0)) {
+                        if (i + 1 < n_here) ok = qk(rt.sees(j0 + KT_TILE), i + 2 == n_here);
+                        ok = ok && wait(&full[vs], vp);
+                        if (ok && i + 1 == n_here && kt_fix(a, KT_TILE, cur.hi - j0)) {
                             ok = wait(&fixed[vs], fp >> vs & 1u);
                             fp ^= 1u << vs;
                         }
+                        if (ok && rt.sees(j0)) {          // O += P · V
+                            ok = wait(&p_full[x][pb], pp >> pb & 1u);
+                            if (!ok) break;
+                            pp ^= 1u << pb;
+                            tc_fence_after();
+                            const uint64_t dv = umma_desc_sw128_mn(ring + vs * UNIT, COL);
+#pragma unroll
+                            for (int k = 0; k < KT_TILE / 16; ++k)
+                                umma_f16_ts(tO, tS + pb * KT_TILE + k * 8, dv + (k * 2048 >> 4), ID_PV, begun || k ? 1u : 0u);
+                            umma_commit(&o_done[x]);
+                            pb ^= 1;
+                            begun = true;
+                        }
                         if (!ok) break;
-                        if (s0) {
-                            ok = wait(&p_full[0], pp0);
-                            if (!ok) break;
-                            pp0 ^= 1;
-                            tc_fence_after();
-                            pv(0, begun0);
-                            begun0 = true;
-                            if (!n0) umma_commit(&o_full[0]);
-                        }
-                        if (n0) qk(0);
-                        if (s1) {
-                            ok = wait(&p_full[1], pp1);
-                            if (!ok) break;
-                            pp1 ^= 1;
-                            tc_fence_after();
-                            pv(1, begun1);
-                            begun1 = true;
-                            if (!n1) umma_commit(&o_full[1]);
-                        }
                         umma_commit(&empty[vs]);
-                        if (n1) qk(1);
-                        if (more) umma_commit(&empty[ks]);
-                        if (i + 2 == n_here) umma_commit(&q_empty);
                         step2(vs, vp);
-                        if (more) step2(ks, kp);
-                        s0 = n0;
-                        s1 = n1;
                     }
                     u += n_here;
                     if (u < u1) cur.next_item(a, Q);
                 }
                 // every MMA issued has finished before the block ends
-                umma_commit(&drain);
-                mbar_wait(&drain, 0);
+                umma_commit(&drain[x]);
+                mbar_wait(&drain[x], 0);
             }
             __syncwarp();
-        } else if (warp == KT_FIXER) {
-            // the V tiles the producer asks for, in its order. A slot asked for is not filled again before
-            // it is cleared, so its barriers are never more than one phase from what is waited for.
-            int asks = 0;
-            for (long u = u0; u < u1;) {
-                if (!begin(u)) break;
-                const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                if (kt_fix(a, KT_TILE, cur.hi - (cur.lo_t + cur.kt + n_here - 1) * KT_TILE)) {
-                    const int at = asks % NU;
-                    if (!kt_wait_warp(&asked[at], (uint32_t)(asks / NU) & 1u, abort_flag, status)) break;
-                    const int slot = s_ask[at][0], end = s_ask[at][2];
-                    if (!kt_wait_warp(&full[slot], (uint32_t)s_ask[at][1], abort_flag, status)) break;
-                    const int rows_z = (end + a.box - 1) / a.box * a.box - end;
-                    for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
-                        const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
-                        *reinterpret_cast<uint4 *>(smem + 2 * QT + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&fixed[slot]);
-                    ++asks;
-                }
-                u += n_here;
-                if (u < u1) cur.next_item(a, Q);
-            }
         }
     } else {
         // ---------------- softmax and output of row tile x, one thread per row
@@ -307,145 +286,92 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lanes + x * 128, tO = tmem + lanes + 256 + x * 128;
         const int tok = row / G, g = row - tok * G;
-        uint32_t sp = 0, op = 0;
+        uint32_t sp = 0, buf = 0, given = 0;              // parity bits of the two S, the next one, P handed over so far
         for (long u = u0; u < u1;) {
             if (!begin(u)) break;
             const KtRows rt(a, cur, Q, x);
             const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
             const int first = (cur.lo_t + cur.kt) * KT_TILE;
             const bool live = tok < rt.t1 - rt.t0 && row < TT * G;
-            const int p = live ? cur.s.p0 + rt.t0 + tok : rt.hi - 1;      // this row's position
+            const int p0 = cur.s.p0 + rt.t0, p = live ? p0 + tok : rt.hi - 1;             // the tile's first, this row's position
             float m = -INFINITY, l = 0.0f;
             bool begun = false;
             for (int i = 0; i < n_here; ++i) {
                 const int j0 = first + i * KT_TILE;
                 if (!rt.sees(j0)) continue;
-                kt_wait(&s_full[x], sp, abort_flag, status);
-                sp ^= 1;
+                const uint32_t tP = tS + buf * KT_TILE;
+                kt_wait(&s_full[x][buf], sp >> buf & 1u, abort_flag, status);
+                sp ^= 1u << buf;
                 tc_fence_after();
-                // some row of the tile does not see all 128
-                const bool edge = j0 + KT_TILE > cur.s.p0 + rt.t0 + 1 || (a.window && j0 < rt.hi - a.window);
-                const int top_j = p - j0, bottom_j = a.window ? top_j - a.window : -1;
+                uint32_t s[KT_TILE];
+                tmem_ld32_nowait(tP, s);
+                tmem_ld32_nowait(tP + 32, s + 32);
+                tmem_wait_ld();
+                settle32(s);
+                settle32(s + 32);
+                if (j0 + KT_TILE > p0 + 1 || (a.window && j0 < rt.hi - a.window)) {
+                    // some row of the tile does not see all 64
+                    const int top = min(p - j0, 63), bottom = a.window ? max(p - a.window - j0, -1) : -1;
+                    const uint64_t seen = top < 0 ? 0ull : (~0ull >> (63 - top)) & (bottom >= 63 ? 0ull : ~0ull << (bottom + 1));
+#pragma unroll
+                    for (int e = 0; e < KT_TILE; ++e)
+                        if (!(seen >> e & 1)) s[e] = 0xff800000u;
+                }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                // scores of 16 columns from c that the row does not see
-                auto hide = [&](uint32_t *v, int c) {
-                    const int up = min(max(top_j + 1 - c, 0), 16), dn = min(max(bottom_j + 1 - c, 0), 16);
-                    const uint32_t seen = ((1u << up) - 1u) & ~((1u << dn) - 1u);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (!(seen >> e & 1u)) v[e] = 0xff800000u;
-                };
-                // weights of 16 scores -> 8 packed pairs; their sum added to `add`
-                const f32x2 scale22 = pack2(a.scale2, a.scale2);
-                auto weigh = [&](const uint32_t *v, f32x2 minus, uint32_t *pk, f32x2 (&add)[2]) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const f32x2 x = fma2(pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale22, minus);
-                        float e0, e1;
-                        unpack2(x, e0, e1);
-                        e0 = ex2(e0);
-                        e1 = ex2(e1);
-                        add[e & 1] = add2(add[e & 1], pack2(e0, e1));
-                        uint32_t w[1];
-                        split_pair<HALF, 1>(e0, e1, w);
-                        pk[e] = w[0];
-                    }
-                };
-                auto largest = [&](const uint32_t *v) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2)
-                        mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                };
-                // O and l to the scale of a larger maximum
-                auto raise = [&](float top) {
-                    const bool grow = top > m + 8.0f;
-                    if (!__any_sync(0xffffffffu, grow)) return false;
+                for (int e = 0; e < KT_TILE; e += 2)
+                    mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+                const bool grow = top > m + 8.0f;
+                if (__any_sync(0xffffffffu, grow)) {      // O and l to the scale of a larger maximum
                     const float f = grow ? ex2(m - top) : 1.0f;
                     if (grow) {
                         m = top;
                         l *= f;
                     }
-                    if (begun) {                          // O holds sums (an item's first product sets it)
+                    if (begun) {                          // once its last product has finished
+                        kt_wait(&o_done[x], (given - 1) & 1u, abort_flag, status);
+                        tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16_nowait(tO + c, o);
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32_nowait(tO + c, o);
                             tmem_wait_ld();
-                            settle16(o);
+                            settle32(o);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st16(tO + c, o);
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st32(tO + c, o);
                         }
-                    }
-                    return true;
-                };
-                auto top_of = [&]() { return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2; };
-                if (!begun) {                             // nothing is known of the maximum yet
-                    uint32_t s[2][32];
-                    tmem_ld32_nowait(tS, s[0]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t *const v = s[c & 1];
-                        tmem_wait_ld();
-                        settle32(v);
-                        if (c < 3) tmem_ld32_nowait(tS + 32 * (c + 1), s[(c + 1) & 1]);
-                        if (edge) {
-                            hide(v, 32 * c);
-                            hide(v + 16, 32 * c + 16);
-                        }
-                        largest(v);
-                        largest(v + 16);
-                    }
-                    raise(top_of());
-                }
-                f32x2 add[2] = {0, 0};
-                uint32_t pk[64];                          // kept until m has proved large enough
-                {
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    const f32x2 minus = pack2(-base, -base);
-                    uint32_t s[2][16];
-                    tmem_ld16_nowait(tS, s[0]);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {         // 16 columns while the next 16 are on their way
-                        uint32_t *const v = s[c & 1];
-                        tmem_wait_ld();
-                        settle16(v);
-                        if (c < 7) tmem_ld16_nowait(tS + 16 * (c + 1), s[(c + 1) & 1]);
-                        if (edge) hide(v, 16 * c);
-                        largest(v);
-                        weigh(v, minus, pk + 8 * c, add);
-                    }
-                }
-                if (!raise(top_of())) {
-                    tmem_st32(tS, pk);
-                    tmem_st32(tS + 32, pk + 32);
-                } else {                                  // rarely: the weights again, with the new maximum
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    const f32x2 minus = pack2(-base, -base);
-                    add[0] = add[1] = 0;
-#pragma unroll 1
-                    for (int c = 0; c < 128; c += 16) {   // P's columns lie behind those of S still to be read
-                        uint32_t v[16], w[8];
-                        tmem_ld16_nowait(tS + c, v);
-                        tmem_wait_ld();
-                        settle16(v);
-                        if (edge) hide(v, c);
-                        weigh(v, minus, w, add);
-                        tmem_st8(tS + c / 2, w);
                     }
                 }
                 begun = true;
+                const float base = m == -INFINITY ? 0.0f : m;
+                const f32x2 minus = pack2(-base, -base), scale22 = pack2(a.scale2, a.scale2);
+                f32x2 add[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < KT_TILE / 2; ++e) {   // the weights, packed into the registers behind
+                    float e0, e1;
+                    unpack2(fma2(pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale22, minus), e0, e1);
+                    e0 = ex2(e0);
+                    e1 = ex2(e1);
+                    add[e & 1] = add2(add[e & 1], pack2(e0, e1));
+                    uint32_t w[1];
+                    split_pair<HALF, 1>(e0, e1, w);
+                    s[e] = w[0];
+                }
+                tmem_st32(tP, s);
                 float a0, a1;
                 unpack2(add2(add[0], add[1]), a0, a1);
                 l += a0 + a1;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+                if (lane == 0) mbar_arrive(&p_full[x][buf]);
+                buf ^= 1;
+                ++given;
             }
             if (begun) {
-                kt_wait(&o_full[x], op, abort_flag, status);
-                op ^= 1;
+                kt_wait(&o_done[x], (given - 1) & 1u, abort_flag, status);
                 tc_fence_after();
             }
 

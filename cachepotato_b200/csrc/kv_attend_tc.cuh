@@ -9,8 +9,7 @@
 namespace cpg {
 
 constexpr int KT_ROWS = 128;                              // rows of an MMA tile
-constexpr int KT_THREADS = 384, KT_PRODUCER = 8, KT_MMA = 9, KT_FIXER = 10;
-constexpr int KT_FIXED = 2;                               // units an item's begin and end are worth (see KD_FIXED)
+constexpr int KT_THREADS = 384, KT_LOAD_K = 8, KT_MMA = 9, KT_LOAD_V = 10;
 template <int HD> constexpr int kt_part() { return (2 + HD) * KT_ROWS; }       // floats of a row tile's part: m, l, o (four columns of a row together)
 
 // Sequence i in units. Group p of its rows (one row tile or a pair) holds tokens [p·Q, min(len, p·Q + Q)).
@@ -25,19 +24,20 @@ __device__ __forceinline__ int kt_tiles(const AttendArgs &a, int Q, const KvSeq 
     const int lo = a.window ? max(0, s.p0 + p * Q - a.window + 1) : 0;
     return (s.p0 + min(s.len, p * Q + Q) - 1) / TILE + 1 - lo / TILE;
 }
-template <int TILE>
+template <int TILE, int FIXED>
 __device__ __forceinline__ KtSeq kt_seq(const AttendArgs &a, int Q, int i) {
     KtSeq q;
     q.s = kv_seq(a.b, a.c.P, i);
     q.pairs = (q.s.len + Q - 1) / Q;
     q.head_units = 0;
     // a handful of instructions a pair; a closed form took longer than summing thousands of pairs
-    for (int p = 0; p < q.pairs; ++p) q.head_units += KT_FIXED + kt_tiles<TILE>(a, Q, q.s, p);
+    for (int p = 0; p < q.pairs; ++p) q.head_units += FIXED + kt_tiles<TILE>(a, Q, q.s, p);
     return q;
 }
 
-// A place in the order of units: sequence, cached head, pair, position tile (kt from -KT_FIXED).
-template <int TILE>
+// A place in the order of units: sequence, cached head, pair, position tile (kt from -FIXED: an item's
+// begin and end are worth FIXED units, see KD_FIXED).
+template <int TILE, int FIXED>
 struct KtCursor {
     int seq, kh, pair, kt;
     KvSeq s;
@@ -52,7 +52,7 @@ struct KtCursor {
         nt = kt_tiles<TILE>(a, Q, s, pair);
     }
     __device__ __forceinline__ void next_item(const AttendArgs &a, int Q) {
-        kt = -KT_FIXED;
+        kt = -FIXED;
         if (++pair < pairs) {
             item(a, Q);
             return;
@@ -71,16 +71,16 @@ struct KtCursor {
 };
 
 // What a block keeps in shared memory of its share.
-template <int TILE>
+template <int TILE, int FIXED>
 struct KtShared {
     long scan[KT_THREADS / 32], off;
     KvCut cut;
-    KtCursor<TILE> cur;
+    KtCursor<TILE, FIXED> cur;
 };
 // This block's range [u0, u1) of all items' units, and in sh.cur the place it starts at, for which the
 // caller's next __syncthreads makes sh ready. false: it has nothing to do (the whole block agrees).
-template <int TILE>
-__device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TILE> &sh, long &u0, long &u1) {
+template <int TILE, int FIXED>
+__device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TILE, FIXED> &sh, long &u0, long &u1) {
     u0 = u1 = 0;
     const int n = a.b.n, blk = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -96,7 +96,7 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
     };
     if (n > KT_THREADS) {                                 // more sequences than threads: their sum first
         long sum = 0;
-        for (int i = tid; i < n; i += KT_THREADS) sum += kt_seq<TILE>(a, Q, i).head_units * a.c.KV;
+        for (int i = tid; i < n; i += KT_THREADS) sum += kt_seq<TILE, FIXED>(a, Q, i).head_units * a.c.KV;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) sh.scan[warp] = sum;
@@ -109,7 +109,7 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
     for (int c0 = 0; c0 < n; c0 += KT_THREADS) {          // THREADS sequences at a time
         KtSeq mine{};
         if (c0 + tid < n) {
-            mine = kt_seq<TILE>(a, Q, c0 + tid);
+            mine = kt_seq<TILE, FIXED>(a, Q, c0 + tid);
             if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
         }
         const long x = mine.head_units * a.c.KV;
@@ -129,7 +129,7 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
         if (n <= KT_THREADS && !range(all)) return false;
         const long at = u0 - (base + inc - x);
         if (at >= 0 && at < x) {
-            KtCursor<TILE> c;
+            KtCursor<TILE, FIXED> c;
             c.seq = c0 + tid;
             c.s = mine.s;
             c.pairs = mine.pairs;
@@ -144,10 +144,10 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
     if (u0 >= u1) return false;                           // no sequences at all
     if (tid == 0) sh.cut = cut;
     if (warp == 0) {                                      // the pair that holds unit sh.off, 32 pairs at a time
-        KtCursor<TILE> c = sh.cur;
+        KtCursor<TILE, FIXED> c = sh.cur;
         long off = sh.off;
         for (int p0 = 0; p0 < c.pairs; p0 += 32) {
-            const int p = p0 + lane, mine = p < c.pairs ? KT_FIXED + kt_tiles<TILE>(a, Q, c.s, p) : 0;
+            const int p = p0 + lane, mine = p < c.pairs ? FIXED + kt_tiles<TILE>(a, Q, c.s, p) : 0;
             int inc = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -158,7 +158,7 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
             if (off < all) {
                 if (off >= inc - mine && off < inc) {
                     c.pair = p;
-                    c.kt = (int)off - (inc - mine) - KT_FIXED;
+                    c.kt = (int)off - (inc - mine) - FIXED;
                     c.item(a, Q);
                     sh.cur = c;
                 }

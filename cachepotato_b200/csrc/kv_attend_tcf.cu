@@ -14,10 +14,9 @@
 //                       terms over S, and the last tile's p·v from TMEM into 128 registers of sums
 //           warps 4-7   f32 cache: the tile that TMA brought into three bf16 planes, 128-byte swizzle;
 //                       places behind the last position become zeros
-//           warp 8      producer (tensor TMA)
+//           warps 8, 10 producers (tensor TMA), as in kv_attend_tc.cu
 //           warp 9      tcgen05.mma: S = q·K^T with q from TMEM, into one of two S while the softmax
 //                       works on the other; p·v
-//           warp 10     16-bit cache: clears places behind the last position (kv_attend_tc.cu)
 //           TMEM: q's terms at 0, S at 192 and 256, P's first two terms over its S, the third at 320,
 //           p·v at 352.
 //   join    Parts of an item that several blocks share, as in kv_attend_tc.cu.
@@ -30,7 +29,7 @@
 
 namespace cpg {
 
-constexpr int KF_TILE = 64;
+constexpr int KF_TILE = 64, KF_FIXED = 2;                 // positions of an MMA tile; units an item's begin and end are worth
 constexpr int KF_S = 192, KF_P3 = 320, KF_O = 352;        // TMEM columns
 template <bool F32C, int HD> constexpr int kf_plane() { return KF_TILE * HD * 2; }                    // one 16-bit plane of a tile
 template <bool F32C, int HD> constexpr int kf_unit() { return KF_TILE * HD * (F32C ? 4 : 2); }        // what TMA brings
@@ -50,18 +49,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
     constexpr uint32_t ID_QK = umma_idesc_f16(128, KF_TILE) | FMT, ID_PV = umma_idesc_f16(128, HD) | FMT | UMMA_B_MN;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t full[NU], empty[NU], asked[NU], fixed[NU], k_full, k_empty, v_full, v_empty, q_full, s_full[2], p_full,
+    __shared__ uint64_t full[NU], empty[NU], fixed[NU], k_full, k_empty, v_full, v_empty, q_full, s_full[2], p_full,
         o_full, drain;
-    __shared__ KtShared<KF_TILE> sh;
+    __shared__ KtShared<KF_TILE, KF_FIXED> sh;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_last, s_ask[NU][3];         // a V tile to clear: ring slot, its fill's parity, first place
+    __shared__ int s_abort, s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = a.H / a.c.KV, TT = KT_ROWS / G;         // tokens of a row tile
     if (tid == 0) {
         for (int i = 0; i < NU; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], F32C ? 4 : 1);
-            mbar_init(&asked[i], 1);
             mbar_init(&fixed[i], 1);
         }
         mbar_init(&k_full, 4);
@@ -83,7 +81,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
     pdl_launch_dependents();
 
     long u0, u1;                                          // this block's range of units
-    if (!kt_begin<KF_TILE>(a, TT, sh, u0, u1)) return;
+    if (!kt_begin<KF_TILE, KF_FIXED>(a, TT, sh, u0, u1)) return;
     if (warp == KT_MMA) {                                 // all of TMEM
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
     int *const status = a.c.status;
     uint8_t *const planes = smem + NU * UNIT;             // K's three, then V's
     const uint32_t ring = smem_u32(smem);
-    KtCursor<KF_TILE> cur = sh.cur;
+    KtCursor<KF_TILE, KF_FIXED> cur = sh.cur;
     // skips an item's fixed share: false if nothing of the item itself is this block's
     auto begin = [&](long &u) {
         if (cur.kt < 0) {
@@ -109,27 +107,35 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
     // registers: the block starts with 384 x 168; 128 threads take 232, 128 keep 168, 128 go down to 104
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == KT_PRODUCER) {
-            // ---------------- producer: lane b loads box b of every unit
+        if (warp == KT_LOAD_K || warp == KT_LOAD_V) {
+            // ---------------- producers of the K and of the V tiles, in turn through the ring (an f32
+            // cache's three slots serve both: one warp loads them). Lane b loads box b of a tile.
+            const int first_half = !F32C && warp == KT_LOAD_V, halves = F32C ? 2 : 1;
             const int boxes = KF_TILE / a.box * PARTS;
-            int slot = 0, turn = 0, asks = 0;
-            bool ok = true;
+            int slot = first_half, turn = 0;
+            bool ok = !F32C || warp == KT_LOAD_K;
+            const bool mine = ok;
             for (long u = u0; u < u1 && ok;) {
                 if (!begin(u)) break;
                 const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u), lo = cur.lo_of(a, cur.pair * TT);
-                for (int i = 0; i < n_here; ++i) {
-                    const int j0 = (cur.lo_t + cur.kt + i) * KF_TILE;
-                    int page = a.c.n_pages, place = 0;    // outside the pool: zeros
-                    const int j = j0 + lane / PARTS * a.box;
-                    if (lane < boxes && j < cur.hi && j + a.box > lo) {
+                // page and place of this lane's box of tile i; the next tile's is asked for ahead
+                auto find = [&](int i, int &page, int &place) {
+                    const int j = (cur.lo_t + cur.kt + i) * KF_TILE + lane / PARTS * a.box;
+                    place = -1;                           // nothing of it is seen
+                    if (lane < boxes && i < n_here && j < cur.hi && j + a.box > lo) {
                         const int pg = j / a.c.P;
-                        const int id = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
-                        if (id >= 0 && id < a.c.n_pages) page = id;
-                        else atomicOr(status, KV_BAD_PAGE);
+                        page = a.b.pages[(size_t)cur.seq * a.b.table_stride + pg];
                         place = j - pg * a.c.P;
                     }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {                // K, then V
+                };
+                int next_page = 0, next_place;
+                find(0, next_page, next_place);
+                for (int i = 0; i < n_here && ok; ++i) {
+                    const bool inside = next_place >= 0 && next_page >= 0 && next_page < a.c.n_pages;
+                    if (next_place >= 0 && !inside) atomicOr(status, KV_BAD_PAGE);
+                    const int page = inside ? next_page : a.c.n_pages, place = max(next_place, 0);   // outside the pool: zeros
+                    find(i + 1, next_page, next_place);
+                    for (int half = first_half; half < first_half + halves; ++half) {     // K, then V
                         ok = !turn || kt_wait_warp(&empty[slot], (uint32_t)(turn - 1) & 1u, abort_flag, status);
                         if (!ok) break;
                         if (lane == 0) mbar_arrive_expect_tx(&full[slot], UNIT);
@@ -137,27 +143,32 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                         if (lane < boxes)
                             tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
                                         lane % PARTS * (128 / ES), place, cur.kh, page, &full[slot]);
-                        if (!F32C && half && kt_fix(a, KF_TILE, cur.hi - j0)) {
-                            if (lane == 0) {
-                                s_ask[asks % NU][0] = slot;
-                                s_ask[asks % NU][1] = turn & 1;
-                                s_ask[asks % NU][2] = cur.hi - j0;
-                                mbar_arrive(&asked[asks % NU]);
+                        // 16-bit cache: clear the places behind the last position (kv_attend_tc.cu)
+                        const int end = cur.hi - (cur.lo_t + cur.kt + i) * KF_TILE;
+                        if (!F32C && half && kt_fix(a, KF_TILE, end)) {
+                            ok = kt_wait_warp(&full[slot], (uint32_t)turn & 1u, abort_flag, status);
+                            if (!ok) break;
+                            const int rows_z = (end + a.box - 1) / a.box * a.box - end;
+                            for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
+                                const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
+                                *reinterpret_cast<uint4 *>(smem + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
                             }
-                            ++asks;
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&fixed[slot]);
                         }
-                        if (++slot == NU) {
-                            slot = 0;
+                        slot += 3 - halves;
+                        if (slot >= NU) {
+                            slot -= NU;
                             ++turn;
                         }
                     }
-                    if (!ok) break;
                 }
                 u += n_here;
                 if (u < u1) cur.next_item(a, TT);
             }
-            if (*abort_flag) {                            // copies in flight land before the block may end
-                for (int i = 0; i < NU; ++i) {
+            if (mine && !ok) {                            // copies in flight land before the block may end
+                for (int i = first_half; i < NU; i += 3 - halves) {
                     const int fills = turn + (i < slot);
                     if (fills) mbar_wait(&full[i], (uint32_t)(fills - 1) & 1u);
                 }
@@ -244,30 +255,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                 mbar_wait(&drain, 0);
             }
             __syncwarp();
-        } else if (!F32C && warp == KT_FIXER) {
-            // the V tiles the producer asks for (kv_attend_tc.cu)
-            int asks = 0;
-            for (long u = u0; u < u1;) {
-                if (!begin(u)) break;
-                const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                if (kt_fix(a, KF_TILE, cur.hi - (cur.lo_t + cur.kt + n_here - 1) * KF_TILE)) {
-                    const int at = asks % NU;
-                    if (!kt_wait_warp(&asked[at], (uint32_t)(asks / NU) & 1u, abort_flag, status)) break;
-                    const int slot = s_ask[at][0], end = s_ask[at][2];
-                    if (!kt_wait_warp(&full[slot], (uint32_t)s_ask[at][1], abort_flag, status)) break;
-                    const int rows_z = (end + a.box - 1) / a.box * a.box - end;
-                    for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
-                        const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
-                        *reinterpret_cast<uint4 *>(smem + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&fixed[slot]);
-                    ++asks;
-                }
-                u += n_here;
-                if (u < u1) cur.next_item(a, TT);
-            }
         }
     } else if (warp >= 4) {
         if constexpr (F32C) {
