@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
     constexpr uint32_t ID_QK = umma_idesc_f16(128, KT_TILE) | FMT, ID_PV = umma_idesc_f16(128, HD) | FMT | UMMA_B_MN;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, fixed[NU], s_full[2][2], p_full[2][2], o_done[2],
-        drain[2];
+    __shared__ uint64_t full[NU], empty[NU], q_full, q_empty, fixed[NU], s_full[2][2], p_full[2][2],
+        o_done[2][2], drain[2];
     __shared__ KtShared<KT_TILE, KT_FIXED> sh;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_last[2];
@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&s_full[x][b], 1);
                 mbar_init(&p_full[x][b], 4);
+                mbar_init(&o_done[x][b], 1);
             }
-            mbar_init(&o_done[x], 1);
         }
         mbar_init(&drain[0], 1);
         mbar_init(&drain[1], 1);
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
 #pragma unroll
                             for (int k = 0; k < KT_TILE / 16; ++k)
                                 umma_f16_ts(tO, tS + pb * KT_TILE + k * 8, dv + (k * 2048 >> 4), ID_PV, begun || k ? 1u : 0u);
-                            umma_commit(&o_done[x]);
+                            umma_commit(&o_done[x][pb]);
                             pb ^= 1;
                             begun = true;
                         }
@@ -286,7 +286,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lanes + x * 128, tO = tmem + lanes + 256 + x * 128;
         const int tok = row / G, g = row - tok * G;
-        uint32_t sp = 0, buf = 0, given = 0;              // parity bits of the two S, the next one, P handed over so far
+        uint32_t given = 0;                               // P handed over so far: P number n lies over S n % 2
+        // P number n has been multiplied. A barrier for each of the two P, and each is waited for before
+        // its next P is written: a parity tells two phases apart, and the softmax may be two P ahead of
+        // the products when V tiles come late (one barrier let it read O too early then).
+        auto done = [&](uint32_t n) { kt_wait(&o_done[x][n & 1], n >> 1 & 1u, abort_flag, status); };
         for (long u = u0; u < u1;) {
             if (!begin(u)) break;
             const KtRows rt(a, cur, Q, x);
@@ -299,9 +303,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
             for (int i = 0; i < n_here; ++i) {
                 const int j0 = first + i * KT_TILE;
                 if (!rt.sees(j0)) continue;
-                const uint32_t tP = tS + buf * KT_TILE;
-                kt_wait(&s_full[x][buf], sp >> buf & 1u, abort_flag, status);
-                sp ^= 1u << buf;
+                const uint32_t buf = given & 1, tP = tS + buf * KT_TILE;
+                kt_wait(&s_full[x][buf], given >> 1 & 1u, abort_flag, status);
+                if (given >= 2) done(given - 2);          // has come with this S; see above
                 tc_fence_after();
                 uint32_t s[KT_TILE];
                 tmem_ld32_nowait(tP, s);
@@ -330,7 +334,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         l *= f;
                     }
                     if (begun) {                          // once its last product has finished
-                        kt_wait(&o_done[x], (given - 1) & 1u, abort_flag, status);
+                        done(given - 1);
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
@@ -367,11 +371,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[x][buf]);
-                buf ^= 1;
                 ++given;
             }
             if (begun) {
-                kt_wait(&o_done[x], (given - 1) & 1u, abort_flag, status);
+                done(given - 1);
                 tc_fence_after();
             }
 

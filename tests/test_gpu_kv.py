@@ -500,6 +500,30 @@ def test_attend_is_the_same_every_time():
                 assert torch.equal(cache.attend(batch, q, ws=ws), first)
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("window", [0, 200])
+def test_attend_when_tiles_come_late(rt, ct, window):
+    """Pages out of memory instead of the L2 cache: tiles of keys and values arrive late and in no order,
+    and every stage of the kernels waits for every other at some time. The same bits each time."""
+    from cachepotato_b200.kv import KVCache
+    lens = [(100 + 9 * i, 37 * i) for i in range(24)] + [(1, 900), (520, 0)]
+    b = R.Batch(lens, 16, 12)
+    kp, vp = R.pools(b, 2, 128, TYPES[ct], 13)
+    poison(b, kp, vp)
+    q = rows((b.rows, 16, 128), TYPES[rt], 14)
+    want, size = R.attend(b, q, kp, vp, 128 ** -0.5, window)
+    cache, batch = KVCache(kp, vp, rope_dim=0), b.device(520)
+    other = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = None
+    for i in range(20):
+        other.fill_(i)                                            # more than L2 holds
+        got = cache.attend(batch, q, window=window)
+        first = got.clone() if first is None else first
+        assert torch.equal(got, first), i
+    close(first, want, attend_tol(b, want, size, vp, TYPES[rt]), "late tiles")
+    cache.check()
+
+
 def test_long_cache_offsets_past_32_bits():
     """A pool of more than 2^32 elements: the last pages are reached."""
     from cachepotato_b200.kv import KVCache
