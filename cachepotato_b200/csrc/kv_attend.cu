@@ -741,10 +741,8 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             auto join = [&](int *counter, int first, int step, int count) -> bool {
                 named_bar_sync(1, KD_WARPS * 32);
                 if (tid == 0) {
-                    __threadfence();
-                    const int last = atomicAdd(counter, 1) == count - 1;
+                    const int last = kv_arrive(counter) == count - 1;
                     if (last) *counter = 0;               // ready for the next call
-                    __threadfence();
                     s_last = last;
                 }
                 named_bar_sync(1, KD_WARPS * 32);
@@ -790,9 +788,10 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                 return true;
             };
             put(part(p));
-            write = join(a.counters + (gi == 0 ? 2 * b0 + 1 : 2 * (b0 + gi * gs)), gi * gs, 1, n_in);
+            // (a group of one is joined as it stands)
+            write = n_in == 1 || join(a.counters + (gi == 0 ? 2 * b0 + 1 : 2 * (b0 + gi * gs)), gi * gs, 1, n_in);
             if (write && ng > 1) {
-                put(part(gi * gs));
+                if (n_in > 1) put(part(gi * gs));
                 write = join(a.counters + 2 * KV_MAX_GRID + b0, 0, gs, ng);
             }
         }

@@ -68,4 +68,12 @@ struct KvCut {
     }
 };
 
+// Adds 1 to a counter of parts: what the block wrote before (its barrier passed) is seen by whoever
+// counts after it, and the other way round.
+__device__ __forceinline__ int kv_arrive(int *counter) {
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
+}
+
 }  // namespace cpg

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     load16(c, v);
                     parts.put16(to, c, v);
                 }
-                if (parts.join(a.counters + parts.slot_of(gi * gs) * 2 + x, &s_last[x], gi * gs, 1, n_in, ng == 1, write16) && ng > 1)
+                if ((n_in == 1 || parts.join(a.counters + parts.slot_of(gi * gs) * 2 + x, &s_last[x], gi * gs, 1, n_in, ng == 1, write16)) && ng > 1)
                     parts.join(a.counters + 4 * KV_MAX_GRID + b0 * 2 + x, &s_last[x], 0, gs, ng, true, write16);
             }
             tc_fence_before();

@@ -239,10 +239,8 @@ struct KtParts {
     __device__ __forceinline__ bool join(int *counter, int *s_last, int first, int step, int count, bool last, Write write) const {
         named_bar_sync(1 + x, 128);
         if (row == 0) {
-            __threadfence();
-            const int mine = atomicAdd(counter, 1) == count - 1;
+            const int mine = kv_arrive(counter) == count - 1;
             if (mine) *counter = 0;                       // ready for the next call
-            __threadfence();
             *s_last = mine;
         }
         named_bar_sync(1 + x, 128);

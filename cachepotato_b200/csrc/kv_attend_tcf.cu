@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                 __stcg(to + KT_ROWS + row, l);
 #pragma unroll
                 for (int c = 0; c < HD; c += 16) parts.put16(to, c, o + c);
-                if (parts.join(a.counters + parts.slot_of(gi * gs) * 2, &s_last, gi * gs, 1, n_in, ng == 1, write16) && ng > 1)
+                if ((n_in == 1 || parts.join(a.counters + parts.slot_of(gi * gs) * 2, &s_last, gi * gs, 1, n_in, ng == 1, write16)) && ng > 1)
                     parts.join(a.counters + 4 * KV_MAX_GRID + b0 * 2, &s_last, 0, gs, ng, true, write16);
             }
             if (u < u1) cur.next_item(a, TT);
