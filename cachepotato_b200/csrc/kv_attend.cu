@@ -83,6 +83,23 @@ __device__ __forceinline__ void mma_acc(float (&d)[4], const uint32_t (&a)[4], u
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The terms of a pair of elements as fragment register `at` of the operands, one operand a term. Packed:
+// rows 8.. of the first operand hold the second term of rows 0..7.
+template <bool PACK, int NP, int NQ>
+__device__ __forceinline__ void place_terms(uint32_t (&w)[NP][4], const uint32_t (&tm)[NQ], int at) {
+    if constexpr (PACK) {
+        w[0][at] = tm[0];
+        w[0][at + 1] = tm[1];
+        if constexpr (NP > 1) {
+            w[1][at] = tm[2];
+            w[1][at + 1] = 0u;
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) w[n][at] = tm[n];
+    }
+}
+
 constexpr int KD_WARPS = 4, KD_KEYS = 16, KD_TILE = KD_WARPS * KD_KEYS, KD_ROWS = 16;
 constexpr int KD_THREADS = (KD_WARPS + 1) * 32;
 constexpr int KD_RING = 96 * 1024;
@@ -97,41 +114,44 @@ template <int HD> constexpr int kd_smem() { return 1008 + KD_RING + kd_buf<HD>()
 // Beginning and ending an item takes a block as long as some three tiles (4 us against 1.4 us for 64
 // bf16 positions), so an item counts for KD_FIXED tiles more than it has: without them the blocks
 // that end one item and begin the next finish last (128K positions, one row: 62 us against 53 us).
-constexpr int KD_FIXED = 3;
+constexpr int KD_FIXED = 4;
 struct KdSeq {
     KvSeq s;
     int rt;                          // row tiles
     long units;
 };
 // Row tile r of a sequence: its (row, head) pairs from r0, nr of them, and the positions they see.
+template <int ROWS>
 struct KdRows {
     int r0, nr, lo, hi, lo_t, nt;
     __device__ __forceinline__ KdRows() {}
     __device__ __forceinline__ KdRows(const AttendArgs &a, int G, const KvSeq &s, int r) {
-        r0 = r * KD_ROWS;
-        nr = min(KD_ROWS, s.len * G - r0);
+        r0 = r * ROWS;
+        nr = min(ROWS, s.len * G - r0);
         lo = a.window ? max(0, s.p0 + r0 / G - a.window + 1) : 0;
         hi = s.p0 + (r0 + nr - 1) / G + 1;
         lo_t = lo / KD_TILE;
         nt = (hi + KD_TILE - 1) / KD_TILE - lo_t;
     }
 };
+template <int ROWS>
 __device__ __forceinline__ KdSeq kd_seq(const AttendArgs &a, int G, int i) {
     KdSeq q;
     q.s = kv_seq(a.b, a.c.P, i);
-    q.rt = (int)(((long)q.s.len * G + KD_ROWS - 1) / KD_ROWS);
+    q.rt = (int)(((long)q.s.len * G + ROWS - 1) / ROWS);
     long tiles = 0;
-    for (int r = 0; r < q.rt; ++r) tiles += KD_FIXED + KdRows(a, G, q.s, r).nt;
+    for (int r = 0; r < q.rt; ++r) tiles += KD_FIXED + KdRows<ROWS>(a, G, q.s, r).nt;
     q.units = a.c.KV * tiles;
     return q;
 }
 
 // A place in the order of units: item (seq, row tile, cached head), position tile.
+template <int ROWS>
 struct KdCursor {
     int seq, rt, kh, kt;             // kt from -KD_FIXED
     KvSeq s;
     int n_rt;
-    KdRows r;
+    KdRows<ROWS> r;
     __device__ __forceinline__ void next_item(const AttendArgs &a, int G) {
         kt = -KD_FIXED;
         if (++kh < a.c.KV) return;
@@ -142,19 +162,21 @@ struct KdCursor {
                 if (++seq >= a.b.n) return;
                 s = kv_seq(a.b, a.c.P, seq);
             } while (s.len == 0);
-            n_rt = (int)(((long)s.len * G + KD_ROWS - 1) / KD_ROWS);
+            n_rt = (int)(((long)s.len * G + ROWS - 1) / ROWS);
         }
-        r = KdRows(a, G, s, rt);
+        r = KdRows<ROWS>(a, G, s, rt);
     }
 };
 
-template <typename TI, typename TC, int HD>
+template <typename TI, typename TC, int HD, bool PACK>
 __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_constant__ AttendArgs a,
                                                              const __grid_constant__ CUtensorMap tm_k,
                                                              const __grid_constant__ CUtensorMap tm_v) {
     constexpr bool F32C = std::is_same<TC, float>::value, F32I = std::is_same<TI, float>::value;
     constexpr bool HALF = std::is_same<TC, __half>::value;
     constexpr int NQ = !F32I ? 1 : HALF ? 2 : 3, NK = F32C ? 3 : 1;
+    constexpr int NP = PACK ? NQ - 1 : NQ;                // operands that hold the terms of q or P
+    constexpr int ROWS = PACK ? 8 : KD_ROWS, RL = ROWS / 8;               // rows of a tile; of a lane
     constexpr int ES = (int)sizeof(TC), PARTS = HD * ES / 128, UNIT = KD_TILE * HD * ES;  // 128-byte columns; ring unit
     constexpr int NU = KD_RING / UNIT;
     constexpr int KS = HD / 16, NT = HD / 8;              // k steps of q·k, n tiles of p·v
@@ -163,7 +185,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     uint8_t *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t full[NU], empty[NU];
     __shared__ long s_scan[KD_WARPS + 1], s_off;
-    __shared__ KdCursor s_cur;
+    __shared__ KdCursor<ROWS> s_cur;
     __shared__ int s_last, s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.H / a.c.KV;
@@ -200,7 +222,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     };
     if (n > KD_THREADS) {                                 // more sequences than threads: their sum first
         long sum = 0;
-        for (int i = tid; i < n; i += KD_THREADS) sum += kd_seq(a, G, i).units;
+        for (int i = tid; i < n; i += KD_THREADS) sum += kd_seq<ROWS>(a, G, i).units;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
@@ -214,7 +236,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     for (int c0 = 0; c0 < n; c0 += KD_THREADS) {          // THREADS sequences at a time
         long inc = 0;
         if (c0 + tid < n) {
-            mine = kd_seq(a, G, c0 + tid);
+            mine = kd_seq<ROWS>(a, G, c0 + tid);
             inc = mine.units;
             if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
         }
@@ -234,7 +256,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         }
         if (n <= KD_THREADS && !range(all)) return;
         if (c0 + tid < n && u0 >= base + inc - x && u0 < base + inc) {
-            KdCursor c;
+            KdCursor<ROWS> c;
             c.seq = c0 + tid;
             c.s = mine.s;
             c.n_rt = mine.rt;
@@ -247,13 +269,13 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     }
     if (u0 >= u1) return;                                 // no sequences at all
     if (warp == 0) {                                      // the row tile that holds unit s_off, 32 at a time
-        KdCursor c = s_cur;
+        KdCursor<ROWS> c = s_cur;
         long off = s_off;
         for (int r0 = 0; r0 < c.n_rt; r0 += 32) {
             const int r = r0 + lane;
             int each = 0;
             if (r < c.n_rt) {
-                c.r = KdRows(a, G, c.s, r);
+                c.r = KdRows<ROWS>(a, G, c.s, r);
                 each = KD_FIXED + c.r.nt;
             }
             long inc = (long)each * a.c.KV;
@@ -276,7 +298,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         }
     }
     __syncthreads();
-    KdCursor cur = s_cur;
+    KdCursor<ROWS> cur = s_cur;
     volatile int *const abort_flag = &s_abort;
 
     if (warp == KD_WARPS) {
@@ -361,8 +383,10 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             const int kh = cur.kh;
             float f[2][F32I ? KS : 1][4];
             float up[2];
+            m[1] = -INFINITY;                             // (packed: no rows of these)
+            l[1] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RL; ++r) {
                 const int rr = cur.r.r0 + g + 8 * r;
                 const bool live = g + 8 * r < cur.r.nr;
                 const int tok = rr / G;
@@ -410,9 +434,9 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             if constexpr (F32I) {                         // warp w writes the steps w, w + 4, ... of all terms
 #pragma unroll
                 for (int k4 = 0; k4 < KS / 4; ++k4) {
-                    uint32_t w[NQ][4];
+                    uint32_t w[NP][4];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                    for (int r = 0; r < RL; ++r)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             uint32_t tm[NQ];
@@ -424,11 +448,10 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                                     hi = f[r][4 * k4 + y][2 * x + 1];
                                 }
                             split_pair<HALF, NQ>(lo * up[r], hi * up[r], tm);
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n) w[n][r + 2 * x] = tm[n];
+                            place_terms<PACK>(w, tm, r + 2 * x);
                         }
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n)
+                    for (int n = 0; n < NP; ++n)
                         s_q[(n * KS + 4 * k4 + warp) * 32 + lane] = make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]);
                 }
                 named_bar_sync(1, KD_WARPS * 32);
@@ -456,9 +479,9 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                     // f32 cache: not unrolled, for a short step's time is in fetching its code
 #pragma unroll KU
                     for (int k2 = 0; k2 < KS / 2; ++k2) {     // 32 elements
-                        uint32_t q2[NQ][2][4];
+                        uint32_t q2[NP][2][4];
 #pragma unroll
-                        for (int q = 0; q < NQ; ++q)
+                        for (int q = 0; q < NP; ++q)
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {
                                 if constexpr (NQ == 1) {
@@ -482,7 +505,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                                     mma_acc<HALF>(big[n][0], q2[0][0], b[0], b[1]);
                                     mma_acc<HALF>(big[n][1], q2[0][1], b[2], b[3]);
 #pragma unroll
-                                    for (int q = NQ - 1; q >= 1; --q) {
+                                    for (int q = NP - 1; q >= 1; --q) {
                                         mma_acc<HALF>(low[n], q2[q][0], b[0], b[1]);
                                         mma_acc<HALF>(low[n], q2[q][1], b[2], b[3]);
                                     }
@@ -496,10 +519,16 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                                     split_pair<HALF, NK>(v.x, v.y, b0);
                                     split_pair<HALF, NK>(v.z, v.w, b1);
                                     mma_acc<HALF>(big[n][b], q2[0][b], b0[0], b1[0]);
+                                    if constexpr (PACK) {
+                                        mma_acc<HALF>(low[n], q2[0][b], b0[2], b1[2]);
+                                        mma_acc<HALF>(low[n], q2[1][b], b0[0], b1[0]);
+                                        mma_acc<HALF>(low[n], q2[0][b], b0[1], b1[1]);
+                                    } else {
 #pragma unroll
-                                    for (int d = NK - 1; d >= 1; --d)      // terms of weight 2^-8d
+                                        for (int d = NK - 1; d >= 1; --d)  // terms of weight 2^-8d
 #pragma unroll
-                                        for (int k = 0; k <= d; ++k) mma_acc<HALF>(low[n], q2[d - k][b], b0[k], b1[k]);
+                                            for (int k = 0; k <= d; ++k) mma_acc<HALF>(low[n], q2[d - k][b], b0[k], b1[k]);
+                                    }
                                 }
                             }
                         }
@@ -508,7 +537,11 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[n][e] = (big[n][0][e] + big[n][1][e]) + low[n][e];
+                            for (int e = 0; e < 2 * RL; ++e) {
+                                float small = low[n][e];
+                                if constexpr (PACK) small += (low[n][e + 2] + big[n][0][e + 2]) + big[n][1][e + 2];
+                                s[n][e] = (big[n][0][e] + big[n][1][e]) + small;
+                            }
                     }
                     const int span = (cur.r.nr - 1) / G + 1;    // positions between the tile's rows, at most
                     if (j0 + KD_KEYS > cur.r.hi - span || (a.window && j0 < cur.r.lo + span)) {
@@ -516,13 +549,13 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
+                            for (int e = 0; e < 2 * RL; ++e) {
                                 const int j = j0 + 8 * n + 2 * t + (e & 1), p = p_row[e >> 1];
                                 if (j > p || (a.window && j <= p - a.window)) s[n][e] = -INFINITY;
                             }
                     }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < RL; ++r) {
                         float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -549,15 +582,14 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                         }
                     }
                 } else if (active) {
-                    uint32_t pa[NQ][4];
+                    uint32_t pa[NP][4];
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
+                        for (int r = 0; r < RL; ++r) {
                             uint32_t tm[NQ];
                             split_pair<HALF, NQ>(s[n][2 * r], s[n][2 * r + 1], tm);
-#pragma unroll
-                            for (int q = 0; q < NQ; ++q) pa[q][r + 2 * n] = tm[q];
+                            place_terms<PACK>(pa, tm, r + 2 * n);
                         }
                     // keys 2t, 2t+1, 2t+8, 2t+9 of this lane's fragments that nobody sees
                     bool hide[4];
@@ -570,7 +602,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                     // f32 rows: o = o·c + sum, rounded
                     auto add_to = [&](float (&to)[4], const float (&sum)[4]) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) to[e] = fmaf(to[e], c[e >> 1], sum[e]);
+                        for (int e = 0; e < 2 * RL; ++e) to[e] = fmaf(to[e], c[e >> 1], PACK ? sum[e] + sum[e + 2 & 3] : sum[e]);
                     };
                     if constexpr (!F32C) {
                         const uint32_t k0 = (hide[0] ? 0u : 0xffffu) | (hide[1] ? 0u : 0xffff0000u);
@@ -592,9 +624,9 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                                 for (int x = 0; x < 2; ++x) {
                                     float sum[4];
-                                    mma_new<HALF>(sum, pa[NQ - 1], b[2 * x], b[2 * x + 1]);
+                                    mma_new<HALF>(sum, pa[NP - 1], b[2 * x], b[2 * x + 1]);
 #pragma unroll
-                                    for (int q = NQ - 2; q >= 0; --q) mma_acc<HALF>(sum, pa[q], b[2 * x], b[2 * x + 1]);
+                                    for (int q = NP - 2; q >= 0; --q) mma_acc<HALF>(sum, pa[q], b[2 * x], b[2 * x + 1]);
                                     add_to(o[2 * n2 + x], sum);
                                 }
                             }
@@ -618,11 +650,16 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                                 split_pair<HALF, NK>(v[0][x], v[1][x], b0);
                                 split_pair<HALF, NK>(v[2][x], v[3][x], b1);
                                 float sum[4];
-                                mma_new<HALF>(sum, pa[NK - 1], b0[0], b1[0]);          // smallest products first
+                                mma_new<HALF>(sum, pa[NP - 1], b0[0], b1[0]);          // smallest products first
+                                if constexpr (PACK) {
 #pragma unroll
-                                for (int d = NK - 1; d >= 0; --d)
+                                    for (int k = NK - 1; k >= 0; --k) mma_acc<HALF>(sum, pa[0], b0[k], b1[k]);
+                                } else {
 #pragma unroll
-                                    for (int k = d == NK - 1; k <= d; ++k) mma_acc<HALF>(sum, pa[d - k], b0[k], b1[k]);
+                                    for (int d = NK - 1; d >= 0; --d)
+#pragma unroll
+                                        for (int k = d == NK - 1; k <= d; ++k) mma_acc<HALF>(sum, pa[d - k], b0[k], b1[k]);
+                                }
                                 add_to(o[4 * cb + x], sum);
                             }
                         }
@@ -643,7 +680,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         constexpr int NQT = NT / 4;                       // n tiles of a quarter
         float *const s_m = s_o + kd_buf<HD>() / 4, *const s_l = s_m + KD_JOIN * KD_ROWS;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < RL; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
             if (t == 0) {
@@ -654,7 +691,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         // the largest maximum of n states in s_m, and the sum of s_l for it
         auto common = [&](int n_states) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RL; ++r) {
                 m[r] = -INFINITY;
                 l[r] = 0.0f;
                 for (int k = 0; k < n_states; ++k) m[r] = fmaxf(m[r], s_m[k * KD_ROWS + g + 8 * r]);
@@ -668,7 +705,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             named_bar_sync(1, KD_WARPS * 32);             // and q's terms are no longer read
             common(KD_WARPS);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RL; ++r) {
                 const float f = m[r] == -INFINITY ? 0.0f : ex2(own[r] - m[r]);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
@@ -686,14 +723,14 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                     for (int i = 0; i < NQT / 2; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 2 * RL; ++e)
                             s_o[((w * 3 + (warp < w ? warp : warp - 1)) * (NQT / 2 * 4) + 4 * i + e) * 32 + lane] = o[w * NQT + h * (NQT / 2) + i][e];
                 }
             named_bar_sync(1, KD_WARPS * 32);
 #pragma unroll
             for (int i = 0; i < NQT / 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2 * RL; ++e) {
                     float sum = 0.0f;
 #pragma unroll
                     for (int w = 0; w < KD_WARPS; ++w) {
@@ -726,7 +763,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
             auto put = [&](float *to) {                   // m, l and o in fragment order, a quarter a warp
                 if (warp == 0 && t == 0) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < RL; ++r) {
                         to[g + 8 * r] = m[r];
                         to[KD_ROWS + g + 8 * r] = l[r];
                     }
@@ -735,7 +772,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < NQT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) __stcg(to + (4 * i + e) * 32, oq[i][e]);
+                    for (int e = 0; e < 2 * RL; ++e) __stcg(to + (4 * i + e) * 32, oq[i][e]);
             };
             // parts first, first + step, ... (count of them): joined by the last of their blocks
             auto join = [&](int *counter, int first, int step, int count) -> bool {
@@ -759,14 +796,14 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < NQT; ++i) oq[i][0] = oq[i][1] = oq[i][2] = oq[i][3] = 0.0f;
                 for (int k0 = 0; k0 < count; k0 += F) {
-                    float v[F][NQT][4];
+                    float v[F][NQT][2 * RL];
 #pragma unroll
                     for (int x = 0; x < F; ++x) {
                         const float *src = part(first + min(k0 + x, count - 1) * step) + 2 * KD_ROWS + warp * NQT * 128 + lane;
 #pragma unroll
                         for (int i = 0; i < NQT; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[x][i][e] = e < 2 || cur.r.nr > 8 ? __ldcg(src + (4 * i + e) * 32) : 0.0f;
+                            for (int e = 0; e < 2 * RL; ++e) v[x][i][e] = e < 2 || cur.r.nr > 8 ? __ldcg(src + (4 * i + e) * 32) : 0.0f;
                     }
                     if (k0 == 0) {
                         named_bar_sync(1, KD_WARPS * 32);
@@ -776,7 +813,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                     for (int x = 0; x < F; ++x) {
                         if (k0 + x >= count) break;
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
+                        for (int r = 0; r < RL; ++r) {
                             const float w = m[r] == -INFINITY ? 0.0f : ex2(s_m[(k0 + x) * KD_ROWS + g + 8 * r] - m[r]);
 #pragma unroll
                             for (int i = 0; i < NQT; ++i)
@@ -798,7 +835,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         if (write) {
             const int kh = cur.kh;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RL; ++r) {
                 if (g + 8 * r >= cur.r.nr) continue;
                 const int rr = cur.r.r0 + g + 8 * r, tok = rr / G;
                 TI *dst = (TI *)a.out + (size_t)(cur.s.r0 + tok) * a.out_stride + (size_t)(kh * G + rr - tok * G) * HD;
@@ -847,24 +884,26 @@ size_t kv_attend_ws_bytes(int hd) {
     return KV_PARTS_AT + std::max(parts, kv_attend_tc_part_bytes(hd));
 }
 
-template <typename TI, typename TC, int HD>
+template <typename TI, typename TC, int HD, bool PACK>
 static int launch_kd(const AttendArgs &a, const CUtensorMap *maps, cudaStream_t s) {
     static std::atomic<bool> set[64];                    // once per device
     int dev = 0;
     CPG_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-        const int rc = allow_max_smem((const void *)k_kv_attend<TI, TC, HD>);
+        const int rc = allow_max_smem((const void *)k_kv_attend<TI, TC, HD, PACK>);
         if (rc) return rc;
         if (dev < 64) set[dev].store(true, std::memory_order_release);
     }
     const int grid = std::min(KV_MAX_GRID, 2 * sm_count());
-    const cudaError_t ce = launch_pdl(k_kv_attend<TI, TC, HD>, dim3(grid), dim3(KD_THREADS), (size_t)kd_smem<HD>(), s, a,
+    const cudaError_t ce = launch_pdl(k_kv_attend<TI, TC, HD, PACK>, dim3(grid), dim3(KD_THREADS), (size_t)kd_smem<HD>(), s, a,
                                       maps[0], maps[1]);
     return ce == cudaSuccess ? CPG_OK : cuda_fail(ce, "cpg_kv_attend");
 }
 template <typename TI, typename TC>
-static int launch_hd(int hd, const AttendArgs &a, const CUtensorMap *maps, cudaStream_t s) {
-    return hd == 128 ? launch_kd<TI, TC, 128>(a, maps, s) : launch_kd<TI, TC, 64>(a, maps, s);
+static int launch_hd(int hd, bool pack, const AttendArgs &a, const CUtensorMap *maps, cudaStream_t s) {
+    if constexpr (std::is_same<TI, float>::value)
+        if (pack) return hd == 128 ? launch_kd<TI, TC, 128, true>(a, maps, s) : launch_kd<TI, TC, 64, true>(a, maps, s);
+    return hd == 128 ? launch_kd<TI, TC, 128, false>(a, maps, s) : launch_kd<TI, TC, 64, false>(a, maps, s);
 }
 
 int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &b, const void *q, size_t q_stride,
@@ -884,12 +923,13 @@ int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &
         a.counters += KD_COUNTERS;
         return type == CPG_T_F32 ? kv_attend_tcf_launch(a, m, hd, s) : kv_attend_tc_launch(a, m, hd, s);
     }
+    const bool pack = most * G <= KD_ROWS / 2;
     a.box = std::min(maps.box, KD_TILE);
     if (type == CPG_T_F32)
-        return c.type == CPG_T_F32   ? launch_hd<float, float>(hd, a, m, s)
-               : c.type == CPG_T_F16 ? launch_hd<float, __half>(hd, a, m, s)
-                                     : launch_hd<float, __nv_bfloat16>(hd, a, m, s);
-    return type == CPG_T_F16 ? launch_hd<__half, __half>(hd, a, m, s) : launch_hd<__nv_bfloat16, __nv_bfloat16>(hd, a, m, s);
+        return c.type == CPG_T_F32   ? launch_hd<float, float>(hd, pack, a, m, s)
+               : c.type == CPG_T_F16 ? launch_hd<float, __half>(hd, pack, a, m, s)
+                                     : launch_hd<float, __nv_bfloat16>(hd, pack, a, m, s);
+    return type == CPG_T_F16 ? launch_hd<__half, __half>(hd, pack, a, m, s) : launch_hd<__nv_bfloat16, __nv_bfloat16>(hd, pack, a, m, s);
 }
 
 }  // namespace cpg
