@@ -46,9 +46,10 @@ namespace cpg {
 // row's loads are in flight.
 //
 // Bound by memory: each value is read and written once. What counts is the bytes in flight, so a
-// thread asks for the next row's heads, unconverted, before it works on this one's (without that
-// 16384 rows of 32 + 2·4 heads in bf16 took 111 us instead of 85), and
-// a run is as long as one wave of blocks needs to take all rows.
+// thread asks for the next row's heads, unconverted, before it works on this one's, and a run is as
+// long as one wave of blocks needs to take all rows. Measured: 16384 rows of 32 + 2·4 heads in bf16
+// (336 MB) 85 us, 3.96 TB/s (111 us without asking ahead; 68 us with the norm and the rotation left
+// out, so the rest is their instructions); one row 3.7 us, 64 rows 4.2 us.
 struct AppendArgs {
     KvRows b;
     KvView c;

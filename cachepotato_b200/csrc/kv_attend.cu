@@ -27,6 +27,12 @@
 //           and the groups by the one that finishes last of all: two short steps where one block
 //           reading up to 296 parts took longer than the attention itself. The order of additions
 //           is that of the parts, so results do not depend on which block came last.
+//           What counts the parts is one acquire-release addition: a sequentially consistent fence waits
+//           for the tiles in flight, 15 us where a block ends an item in the middle of its range.
+//   measured  128 bf16 rows over 1000-8000 positions (1.14 GB): 188 us, 0.93 of the copy bandwidth; 64 f32
+//           rows over f16, 128-4096 positions (294 MB): 56 us, 0.80; one bf16 row over 128K positions
+//           (268 MB): 59 us, 0.70 (4.5 us until the first tile, 41 of tiles at the copy bandwidth, the
+//           rest the joins of 74 parts); one f32 row over 512 positions: 11 us.
 //   types   16-bit rows: one product per step, P rounded to the cache's type (its rounding is as
 //           large as the result's own). f32 rows keep about 22 bits: over an f16 cache q (scaled by
 //           a power of two per row) and P are split into two f16 terms; over a bf16 cache into three
@@ -34,7 +40,9 @@
 //           exact) and the six products of weight 2^-16 and more are kept. The tensor core cuts
 //           off what it adds to an accumulator instead of rounding, so for f32 rows an accumulator
 //           takes few steps, the smallest products first, and is added to the running sum by a
-//           rounded f32 addition (errors 2.9e-6 without that, 4e-7 with it).
+//           rounded f32 addition (errors 2.9e-6 without that, 3e-7 with it). Where a tile has at most 8
+//           rows the other 8 of the operand hold the second term of the same rows, and one product
+//           does the work of two (PACK).
 #include <math.h>
 
 #include <algorithm>
@@ -111,9 +119,10 @@ template <int HD> constexpr int kd_buf() { return 3 * HD / 16 * 512; }
 template <int HD> constexpr int kd_smem() { return 1008 + KD_RING + kd_buf<HD>() + KD_JOIN * 2 * KD_ROWS * 4; }
 
 // Sequence i's units: for each row tile, KV · (KD_FIXED + the position tiles its rows see).
-// Beginning and ending an item takes a block as long as some three tiles (4 us against 1.4 us for 64
+// Beginning and ending an item takes a block as long as some four tiles (5 us against 1.4 us for 64
 // bf16 positions), so an item counts for KD_FIXED tiles more than it has: without them the blocks
-// that end one item and begin the next finish last (128K positions, one row: 62 us against 53 us).
+// that end one item and begin the next finish last (64 f32 rows over f16 70 us against 61, 128K
+// positions and one row 63 against 59).
 constexpr int KD_FIXED = 4;
 struct KdSeq {
     KvSeq s;
@@ -912,14 +921,16 @@ int kv_attend_launch(const KvView &c, const KvMaps &maps, int hd, const KvRows &
     AttendArgs a{b, c, q, out, q_stride, out_stride, n_heads, scale * 1.4426950408889634f, window, maps.box,
                  (float *)((uint8_t *)ws + KV_PARTS_AT), (int *)ws};
     const CUtensorMap *m = maps.m;
-    // Past two row tiles of this file's kernel per sequence and cached head the chunk kernels take over:
-    // their 128 or 256 rows share each tile of K and V that is read, but beginning and joining cost
-    // them more. Measured (us, few / chunk, 4 cached heads of 128): 32 rows of one sequence over 4096
-    // positions 17 / 37 in bf16 and 22 / 36 in f32, of 64 sequences over 1000 62 / 56 and 134 / 141;
-    // 64 rows 19 / 36 and 29 / 35, 107 / 54 and 247 / 141.
+    // Past two row tiles of this file's kernel per sequence and cached head, and four in all, the chunk
+    // kernels take over: their 128 or 256 rows share each tile of K and V that is read, but beginning and
+    // joining cost them more. Measured (us, few / chunk, 4 cached heads of 128): 64 rows of one sequence
+    // over 4096 positions 18 / 36 in bf16, 19 / 34 in f32 over f16, 28 / 36 in f32; 128 rows 22 / 36,
+    // 29 / 38, 54 / 39; of 64 sequences over 1000 positions 24 rows 53 / 43, 64 rows 94 / 43 in bf16.
+    // Of single rows (up to eight per cached head) f32 ones are packed: 64 rows over f16 56 us instead
+    // of 61, one row over 512 f32 positions 11.2 instead of 13.5.
     const int G = n_heads / c.KV;
     const long most = max_new > 0 ? std::min(max_new, b.T) : b.T;
-    if (G <= 128 && most * G > 2 * KD_ROWS) {
+    if (G <= 128 && most * G > 2 * KD_ROWS && (long)b.T * G > 4 * KD_ROWS) {
         a.counters += KD_COUNTERS;
         return type == CPG_T_F32 ? kv_attend_tcf_launch(a, m, hd, s) : kv_attend_tc_launch(a, m, hd, s);
     }

@@ -20,6 +20,9 @@
 //           TMEM: q's terms at 0, S at 192 and 256, P's first two terms over its S, the third at 320,
 //           p·v at 352.
 //   join    Parts of an item that several blocks share, as in kv_attend_tc.cu.
+//   measured  512 f32 rows of 32 heads over themselves, f32 cache (2.1 GFLOP, six times that in bf16
+//           products): 40 us: 2.5 us to the block's range, 4 us for q's terms, 3.3 us a tile (softmax,
+//           p·v and its collection wait for one another), 3.5 us to end an item.
 #include <math.h>
 
 #include <algorithm>
