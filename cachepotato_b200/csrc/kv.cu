@@ -327,6 +327,7 @@ static int kv_create(const cpg_kv_desc *d, const cpg_kv *like, cpg_kv **out) {
     if (ce != cudaSuccess) {
         if (kv->owns) cudaFree(kv->v.status);
         delete kv;
+        cudaGetLastError();                              // reported; the next launch's check does not see it
         return cuda_fail(ce, "cpg_kv_create");
     }
     *out = kv;

@@ -1638,20 +1638,35 @@ extern "C" int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, in
     CPG_REQUIRE(page_size >= 8 && page_size % 8 == 0 && page_size <= 65536, "%s: page_size %d (a multiple of 8, at most 65536)", fn, page_size);
     CPG_REQUIRE(n_pages >= 1, "%s: n_pages %d", fn, n_pages);
     CPG_REQUIRE(type == CPG_T_F32 || type == CPG_T_F16 || type == CPG_T_BF16, "%s: element type %d", fn, type);
+    const size_t S = n_slots, es = type == CPG_T_F32 ? 4 : 2, KD = (size_t)m->KV * QW_HD;
+    const double bytes = 2.0 * m->L * n_pages * page_size * KD * es;
+    if (bytes > 1e13) {                                  // before the product below passes 64 bits
+        set_error("%s: %d pages of %d positions are %.3g bytes", fn, n_pages, page_size, bytes);
+        return CPG_ENOMEM;
+    }
+    const size_t one = (size_t)n_pages * page_size * KD * es;
     cpg_qwen3_paged *p = new (std::nothrow) cpg_qwen3_paged();
-    if (!p) {
+    bool ok = p != nullptr;
+    if (ok) {
+        try {
+            p->pos.assign(n_slots, -1);
+            p->held.resize(n_slots);
+            p->graphs.assign(n_slots + 1, nullptr);
+            p->kv.reserve(m->L);
+            p->free_pages.reserve(n_pages);              // a dropped slot's pages come back without an allocation
+            for (int i = n_pages - 1; i >= 0; --i) p->free_pages.push_back(i);
+        } catch (const std::bad_alloc &) {
+            delete p;
+            ok = false;
+        }
+    }
+    if (!ok) {
         set_error("%s: host allocation failed", fn);
         return CPG_ENOMEM;
     }
     p->m = m;
     p->S = n_slots; p->C = max_ctx; p->P = page_size; p->n_pages = n_pages;
     p->W = (max_ctx + page_size - 1) / page_size;
-    p->pos.assign(n_slots, -1);
-    p->held.resize(n_slots);
-    p->graphs.assign(n_slots + 1, nullptr);
-    for (int i = n_pages - 1; i >= 0; --i) p->free_pages.push_back(i);
-    const size_t S = n_slots, es = type == CPG_T_F32 ? 4 : 2, KD = (size_t)m->KV * QW_HD;
-    const size_t one = (size_t)n_pages * page_size * KD * es;
     const size_t in_ints = 3 * S + 1 + S * p->W;
     cudaError_t ce = cudaMalloc(&p->pool, (size_t)m->L * 2 * one);
     if (ce == cudaSuccess) ce = cudaMalloc(&p->d_step_in, in_ints * sizeof(int));
@@ -1683,6 +1698,7 @@ extern "C" int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, in
     if (!rc && n_slots >= QW_DENSE_DEC_MIN_T && m->dn.attn.empty()) rc = build_dense(m);
     if (rc) {
         paged_free(p);
+        cudaGetLastError();                              // reported; the next launch's check does not see it
         return rc;
     }
     *out = p;
@@ -1698,13 +1714,11 @@ extern "C" void cpg_qwen3_paged_destroy(cpg_qwen3_paged *p) {
 // The named slots: distinct, each with room for its new rows; pages for all of them, or none taken.
 static int paged_reserve(cpg_qwen3_paged *p, const int *slots, const int *n_new, int n, int every, const char *fn) {
     CPG_REQUIRE(slots && n >= 1 && n <= p->S, "%s: %d sequences (1..%d)", fn, n, p->S);
-    std::vector<char> seen(p->S, 0);
     long need = 0;
     for (int i = 0; i < n; ++i) {
         const int j = slots[i], c = n_new ? n_new[i] : every;
         CPG_REQUIRE(j >= 0 && j < p->S, "%s: slot %d of %d", fn, j, p->S);
-        CPG_REQUIRE(!seen[j], "%s: slot %d named twice", fn, j);
-        seen[j] = 1;
+        CPG_REQUIRE(std::find(slots, slots + i, j) == slots + i, "%s: slot %d named twice", fn, j);
         CPG_REQUIRE(c >= 1, "%s: slot %d takes %d tokens", fn, j, c);
         CPG_REQUIRE(n_new || p->pos[j] >= 1, "%s: slot %d holds no sequence", fn, j);
         const long to = (long)std::max(p->pos[j], 0) + c;
@@ -1715,9 +1729,15 @@ static int paged_reserve(cpg_qwen3_paged *p, const int *slots, const int *n_new,
         set_error("%s: the step needs %ld more pages, the pool has %zu free", fn, need, p->free_pages.size());
         return CPG_ENOMEM;
     }
+    auto pages_of = [&](int i) { return (std::max(p->pos[slots[i]], 0) + (n_new ? n_new[i] : every) + p->P - 1) / p->P; };
+    try {
+        for (int i = 0; i < n; ++i) p->held[slots[i]].reserve(pages_of(i));
+    } catch (const std::bad_alloc &) {
+        set_error("%s: host allocation failed", fn);
+        return CPG_ENOMEM;
+    }
     for (int i = 0; i < n; ++i) {
-        const int j = slots[i];
-        const int pages = (std::max(p->pos[j], 0) + (n_new ? n_new[i] : every) + p->P - 1) / p->P;
+        const int j = slots[i], pages = pages_of(i);
         while ((int)p->held[j].size() < pages) {
             p->held[j].push_back(p->free_pages.back());
             p->free_pages.pop_back();

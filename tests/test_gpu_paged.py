@@ -200,3 +200,23 @@ def test_refusals_change_nothing(orc):
     finally:
         p.close()
         gm.close()
+
+
+def test_pools_no_memory_holds(orc):
+    """Sizes past 64 bits are refused before anything is allocated, ones past the device's memory by the
+    allocation; the model goes on."""
+    from cachepotato_b200 import CpgError, _lib
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    m = _small(orc, 71)
+    gm = device_model(m, max_ctx=64)
+    try:
+        for n_pages, page in ((2**31 - 1, 8), (2**31 - 1, 65536), (2000, 65536)):
+            with pytest.raises(CpgError) as e:
+                Qwen3Paged(gm, 2, 64, n_pages=n_pages, page_size=page)
+            assert e.value.code == _lib.CPG_ENOMEM
+        p = Qwen3Paged(gm, 2, 64, n_pages=8, page_size=16)
+        ids = _prompts(m.vocab, [9], 72)[0]
+        assert p.step([1], [ids])[0] == gm.generate(ids, 1)[0]
+        p.close()
+    finally:
+        gm.close()
