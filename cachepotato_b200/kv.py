@@ -123,9 +123,12 @@ class KVCache:
         if q is not None:
             qs, heads = self._rows(q, "q", batch.rows, None), q.shape[1]
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                with torch.cuda.stream(stream):          # memory that is free on the stream that writes it
+                    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             os_ = self._rows(q_out, "q_out", batch.rows, heads)
             _require(q.dtype == dt and q_out.dtype == dt, "q, k, v and q_out must have one type")
+        else:
+            _require(q_out is None, "q_out without q")
         _require(v.dtype == dt, "q, k, v and q_out must have one type")
         for g in (q_norm, k_norm):
             _require(g is None or (g.dtype is torch.float32 and g.shape == (self.head_dim,) and g.is_contiguous()
@@ -143,7 +146,8 @@ class KVCache:
         qs = self._rows(q, "q", batch.rows, None)
         heads = q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            with torch.cuda.stream(stream):              # memory that is free on the stream that writes it
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         os_ = self._rows(out, "out", batch.rows, heads)
         _require(out.dtype == q.dtype, "out and q must have one type")
         if ws is None:

@@ -15,6 +15,7 @@ import pytest
 import torch
 
 import kv_reference as R
+from cachepotato_b200._lib import CpgError
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -484,6 +485,32 @@ def test_two_streams_and_another_stream():
         got = [cache.attend(b.device(1), q, ws=w, stream=s) for q, w, s in zip(qs, wss, streams)]
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_outputs_made_for_another_stream():
+    """What the calls allocate is free on the stream that writes it: not a block that the current stream
+    has given back but is still using."""
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(40, 30), (1, 5)], 16, 3)
+    kp, vp = R.pools(b, 2, 64, torch.float32, 4)
+    cache, batch = KVCache(kp, vp), b.device(40)
+    q, k = rows((b.rows, 8, 64), torch.float32, 5), rows((b.rows, 2, 64), torch.float32, 6)
+    ws = cache.workspace(8)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    given_back = []
+    for _ in range(4):                                            # blocks of the outputs' size, freed on the current stream
+        given_back.append(torch.empty_like(q))
+    places = {t.data_ptr() for t in given_back}
+    del given_back
+    made = cache.append(batch, q, k, k, stream=side)
+    out = cache.attend(batch, made, ws=ws, stream=side)
+    assert made.data_ptr() not in places and out.data_ptr() not in places
+    side.synchronize()
+    want = cache.attend(batch, cache.append(batch, q, k, k), ws=ws)
+    assert torch.equal(out, want)
+    with pytest.raises(CpgError):
+        cache.append(batch, None, k, k, q_out=q)
 
 
 def test_attend_is_the_same_every_time():
