@@ -357,7 +357,8 @@ int cpg_kv_append(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads
  * window > 0 only to j > p - window; n_heads a multiple of n_kv, consecutive heads sharing a cached
  * one; weights softmax(scale q·k). Positions behind a sequence's last row are not looked at,
  * whatever the pages hold there. A position that only some rows of a sequence see takes part in the
- * others' sums with weight zero, so its value must be finite. out may be q.
+ * others' sums with weight zero, so its value must be finite; f32 rows are split into 16-bit terms, so
+ * they and what they see must be finite too. out may be q.
  * f32 rows: products to about 22 bits, f32 sums. 16-bit rows: the weights are rounded to the
  * cache's type before the sum over values, which accumulates in f32.
  * ws: device memory of cpg_kv_attend_workspace_bytes, zeroed once before its first use; every call

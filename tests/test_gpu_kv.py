@@ -228,6 +228,21 @@ def test_attend_any_hint(max_new, rt, ct):
     check_attend([(1, 100), (90, 41), (3, 7)], 16, 8, 2, 128, TYPES[rt], TYPES[ct], max_new=max_new)
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("window", [0, 100])
+def test_attend_chunks_beside_single_rows(rt, ct, window):
+    """A step's single tokens and prompt chunks, lengths on both sides of every choice of kernel between
+    them, empty sequences, more sequences than a block has threads; any hint gives the same rows."""
+    rng = np.random.default_rng(17)
+    some = [(1, int(c)) for c in rng.integers(0, 600, 20)]
+    check_attend(some[:9] + [(200, 333)] + some[9:] + [(0, 9), (3, 50)], 16, 8, 2, 128, TYPES[rt], TYPES[ct], window=window, pad=2)
+    check_attend(some + [(8, 40), (9, 40), (7, 0), (64, 5), (4, 1), (5, 90)], 24, 16, 4, 64, TYPES[rt], TYPES[ct], window=window)
+    many = [(int(n), int(c)) for n, c in zip(rng.integers(0, 3, 450), rng.integers(0, 60, 450))]
+    many[7], many[440] = (150, 20), (33, 70)
+    for max_new in (150, 1, 0):
+        check_attend(many, 8, 4, 2, 64, TYPES[rt], TYPES[ct], window=window, max_new=max_new)
+
+
 @pytest.mark.parametrize("rt,ct", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
 def test_attend_long_and_many(rt, ct):
     check_attend([(1, 20011)], 64, 8, 1, 128, TYPES[rt], TYPES[ct])
