@@ -39,17 +39,18 @@ namespace cpg {
 // exact, and the rest in [-1, 1] goes to sincospif. With rope_f32 it is the reference's arithmetic
 // instead: an f32 frequency, an f32 product.
 //
-// HD / 8 threads hold a head, each two groups of four elements that are rotation partners (elements
-// 4c.. and R/2 + 4c.., c < R / 8; the rest in pairs of neighbours), so nothing crosses lanes but the
-// sum of squares, and a row's sines are the same registers for all of a thread's heads. The rows'
-// places (a search over q_start, then the table) and sines are found once per block, while the first
-// row's loads are in flight.
+// A thread holds two runs of E elements of a head that are rotation partners, 16 bytes of a row each
+// (elements Ec.. and R/2 + Ec.., c < R / 2E; the rest in neighbouring runs), so nothing crosses lanes
+// but the sum of squares, and a row's sines are the same registers for all of a thread's heads. The
+// rows' places (a search over q_start, then the table) and sines are found once per block, while the
+// first row's loads are in flight.
 //
 // Bound by memory: each value is read and written once. What counts is the bytes in flight, so a
 // thread asks for the next row's heads, unconverted, before it works on this one's, and a run is as
 // long as one wave of blocks needs to take all rows. Measured: 16384 rows of 32 + 2·4 heads in bf16
-// (336 MB) 85 us, 3.96 TB/s (111 us without asking ahead; 68 us with the norm and the rotation left
-// out, so the rest is their instructions); one row 3.7 us, 64 rows 4.2 us.
+// (336 MB) 74 us, 4.5 TB/s (8 bytes a load 85 us; without asking ahead as well 111), in f32 (671 MB)
+// 118 us, 5.7 TB/s (32 bytes a load 162: registers for three blocks instead of four); one row 3.6 us,
+// 64 rows 4.1 us.
 struct AppendArgs {
     KvRows b;
     KvView c;
@@ -62,31 +63,43 @@ struct AppendArgs {
     const double *freq;
 };
 
-constexpr int AP_U = 4, AP_MAX_ROWS = 32, AP_BLOCKS = 4;   // query heads of a lane group in flight; rows of a block; blocks per SM
+constexpr int AP_MAX_ROWS = 32, AP_BLOCKS = 4;            // rows of a block; blocks per SM
 
-// Four elements as they lie in memory, and as f32.
-template <typename T> struct Quad;
-template <> struct Quad<float> { using type = float4; };
-template <> struct Quad<__half> { using type = uint2; };
-template <> struct Quad<__nv_bfloat16> { using type = uint2; };
+// N elements, four at a time, and a store of all of them at once (as it lies in memory: 8, 16 or 32 bytes).
+template <int N, typename T>
+__device__ __forceinline__ void get(const T *p, float *y) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) load4(p + i, y + i);
+}
+template <int N, typename T>
+__device__ __forceinline__ void put(T *p, const float *y) {
+    struct alignas(N * sizeof(T) < 16 ? 8 : 16) Run { T v[N]; } o;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) store4(o.v + i, y + i);
+    *reinterpret_cast<Run *>(p) = o;
+}
 
 template <typename TI, typename TC, int HD>
 __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_constant__ AppendArgs a) {
-    using Raw = typename Quad<TI>::type;
+    using Raw = uint4;                                    // as it lies in memory
     pdl_wait();
     pdl_launch_dependents();
-    constexpr int TPH = HD / 8, HPW = 32 / TPH;           // threads per head, heads per warp
-    extern __shared__ float2 s_cs[];                      // (rows, R / 2)
+    constexpr int E = sizeof(Raw) / sizeof(TI);           // elements of a load
+    constexpr int TPH = HD / (2 * E), HPW = 32 / TPH;     // threads per head, heads per warp
+    constexpr int AP_U = 16 / E;                          // query heads of a lane group in flight
+    extern __shared__ float4 s_cs[];                      // a row's R / 4: pairs Ec + 2i, Ec + 2i + 1 at i·R/2E + c
     __shared__ int s_pos[AP_MAX_ROWS], s_page[AP_MAX_ROWS];   // position, -1: no sequence's row; page, -1: none
     const int t0 = blockIdx.x * a.rows, rows = min(a.rows, a.b.T - t0);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int KV = a.c.KV, R = a.R;
     const int sub = lane % TPH;
-    const bool turns = sub < R / 8;
-    const int ea = turns ? 4 * sub : 8 * sub, eb = ea + (turns ? R / 2 : 4);   // 8·sub = R + 8·(sub - R/8)
+    const bool turns = sub < R / (2 * E);
+    const int ea = turns ? E * sub : 2 * E * sub, eb = ea + (turns ? R / 2 : E);   // 2E·sub = R + 2E·(sub - R/2E)
     // lane groups of a row, over all its blocks: group `grp` takes the heads grp, grp + groups, ...
     const int groups = gridDim.y * (blockDim.x >> 5) * HPW;
     const int grp = (blockIdx.y * (blockDim.x >> 5) + warp) * HPW + lane / TPH;
+    // keys and values change sides with every row: they are fewer than the lane groups
+    auto kv_grp = [&](int t) { return t & 1 ? (grp < groups / 2 ? grp + groups - groups / 2 : grp - groups / 2) : grp; };
 
     // a row's query heads from h, and its key or value head h
     auto load_q = [&](Raw (&x)[AP_U][2], int t, int h) {
@@ -107,7 +120,7 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
     };
     Raw nq[AP_U][2], nkv[2];                              // the next row's
     load_q(nq, t0, grp);
-    load_kv(nkv, t0, grp);
+    load_kv(nkv, t0, kv_grp(t0));
 
     for (int r = warp; r < rows; r += blockDim.x >> 5) {
         const int t = t0 + r, i = kv_find_seq(a.b.q_start, a.b.n, t);
@@ -133,11 +146,12 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
             s_page[r] = page;
         }
     }
-    float gq[8];
-    if (a.q_norm) {
-        load4(a.q_norm + ea, gq);
-        load4(a.q_norm + eb, gq + 4);
-    }
+    float gq[2 * E];
+    auto gains = [&](const float *g, float *to) {
+        get<E>(g + ea, to);
+        get<E>(g + eb, to + E);
+    };
+    if (a.q_norm) gains(a.q_norm, gq);
     __syncthreads();
     for (int z = tid; z < rows * (R / 2); z += blockDim.x) {
         const int r = z / (R / 2), j = z - r * (R / 2), pos = s_pos[r];
@@ -150,21 +164,21 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
             const double turn = (double)pos * __ldg(a.freq + j);
             sincospif((float)(turn - 2.0 * rint(0.5 * turn)), &sn, &cs);
         }
-        s_cs[z] = make_float2(cs, sn);
+        reinterpret_cast<float2 *>(s_cs)[r * (R / 2) + 2 * (j % E / 2 * (R / (2 * E)) + j / E) + (j & 1)] = make_float2(cs, sn);
     }
     __syncthreads();
     // the sums below are among the threads of one head, which agree on everything that branches
     const unsigned mask = ((1u << TPH) - 1u) << (lane / TPH * TPH);
 
-    auto norm = [&](float (&y)[8], const float (&g)[8]) {
+    auto norm = [&](float (&y)[2 * E], const float (&g)[2 * E]) {
         float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+        for (int i = 0; i < 2 * E; ++i) ss = fmaf(y[i], y[i], ss);
 #pragma unroll
         for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
         const float inv = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= inv * g[i];
+        for (int i = 0; i < 2 * E; ++i) y[i] *= inv * g[i];
     };
     for (int r = 0; r < rows; ++r) {
         const int t = t0 + r, pos = s_pos[r], page = s_page[r];
@@ -178,21 +192,22 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
         xkv[1] = nkv[1];
         if (r + 1 < rows) {
             load_q(nq, t + 1, grp);
-            load_kv(nkv, t + 1, grp);
+            load_kv(nkv, t + 1, kv_grp(t + 1));
         }
         if (pos < 0) continue;                            // a row of no sequence
-        float2 cs[4] = {};
+        float4 cs[E / 2] = {};
         if (turns) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) cs[i] = s_cs[r * (R / 2) + 4 * sub + i];
+            for (int i = 0; i < E / 2; ++i) cs[i] = s_cs[r * (R / 4) + i * (R / (2 * E)) + sub];
         }
-        auto turn = [&](float (&y)[8]) {
+        auto turn = [&](float (&y)[2 * E]) {
             if (!turns) return;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float lo = y[i], hi = y[4 + i];
-                y[i] = fmaf(lo, cs[i].x, -(hi * cs[i].y));
-                y[4 + i] = fmaf(hi, cs[i].x, lo * cs[i].y);
+            for (int i = 0; i < E; ++i) {
+                const float c = i & 1 ? cs[i / 2].z : cs[i / 2].x, sn = i & 1 ? cs[i / 2].w : cs[i / 2].y;
+                const float lo = y[i], hi = y[E + i];
+                y[i] = fmaf(lo, c, -(hi * sn));
+                y[E + i] = fmaf(hi, c, lo * sn);
             }
         };
         for (int h = grp;;) {
@@ -200,13 +215,13 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
 #pragma unroll
             for (int u = 0; u < AP_U; ++u)
                 if (h + u * groups < a.H) {
-                    float y[8];
-                    load4(reinterpret_cast<const TI *>(&xq[u][0]), y);
-                    load4(reinterpret_cast<const TI *>(&xq[u][1]), y + 4);
+                    float y[2 * E];
+                    get<E>(reinterpret_cast<const TI *>(&xq[u][0]), y);
+                    get<E>(reinterpret_cast<const TI *>(&xq[u][1]), y + E);
                     if (a.q_norm) norm(y, gq);
                     turn(y);
-                    store4(dst + u * groups * HD + ea, y);
-                    store4(dst + u * groups * HD + eb, y + 4);
+                    put<E>(dst + u * groups * HD + ea, y);
+                    put<E>(dst + u * groups * HD + eb, y + E);
                 }
             h += AP_U * groups;
             if (h >= a.H) break;
@@ -214,23 +229,22 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
         }
         if (page < 0) continue;
         const size_t place = (size_t)page * a.c.sp + (size_t)(pos % a.c.P) * a.c.st;
-        for (int h = grp; h < 2 * KV;) {                  // keys, then values
+        for (int h = kv_grp(t); h < 2 * KV;) {                  // keys, then values
             const bool isk = h < KV;
-            float y[8];
-            load4(reinterpret_cast<const TI *>(&xkv[0]), y);
-            load4(reinterpret_cast<const TI *>(&xkv[1]), y + 4);
+            float y[2 * E];
+            get<E>(reinterpret_cast<const TI *>(&xkv[0]), y);
+            get<E>(reinterpret_cast<const TI *>(&xkv[1]), y + E);
             if (isk) {
                 if (a.k_norm) {
-                    float gk[8];
-                    load4(a.k_norm + ea, gk);
-                    load4(a.k_norm + eb, gk + 4);
+                    float gk[2 * E];
+                    gains(a.k_norm, gk);
                     norm(y, gk);
                 }
                 turn(y);
             }
             TC *to = (TC *)(isk ? a.c.k : a.c.v) + place + (size_t)(isk ? h : h - KV) * a.c.sh;
-            store4(to + ea, y);
-            store4(to + eb, y + 4);
+            put<E>(to + ea, y);
+            put<E>(to + eb, y + E);
             h += groups;
             load_kv(xkv, t, h);
         }
@@ -392,9 +406,9 @@ extern "C" int cpg_kv_append(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     a.eps = eps; a.theta = kv->theta;
     a.H = n_heads; a.R = kv->rope_dim; a.rope_f32 = kv->rope_f32;
     a.freq = (const double *)((const char *)kv->v.status + offsetof(KvDevice, freq));
-    // Many rows: runs that one wave of AP_BLOCKS blocks per SM takes, four warps each. Few rows: one a
+    // Many rows: runs that one wave of blocks takes, four warps each. Few rows: one a
     // block, and a row over several blocks while the rows alone leave SMs idle.
-    const int per_warp = 256 / kv->hd, heads = std::max(n_heads, 2 * kv->v.KV), sms = sm_count();
+    const int per_warp = (type == CPG_T_F32 ? 256 : 512) / kv->hd, heads = std::max(n_heads, 2 * kv->v.KV), sms = sm_count();
     a.rows = std::min(AP_MAX_ROWS, (a.b.T + sms * AP_BLOCKS - 1) / (sms * AP_BLOCKS));
     int split = 1;
     while (split < 8 && (long)a.b.T * split < sms && heads > split * 4 * per_warp) split *= 2;
