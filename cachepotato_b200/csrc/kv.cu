@@ -65,7 +65,7 @@ struct AppendArgs {
 
 constexpr int AP_MAX_ROWS = 32, AP_BLOCKS = 4;            // rows of a block; blocks per SM
 
-// N elements, four at a time, and a store of all of them at once (as it lies in memory: 8, 16 or 32 bytes).
+// N elements, four at a time, and a store of all of them at once (8 or 16 bytes).
 template <int N, typename T>
 __device__ __forceinline__ void get(const T *p, float *y) {
 #pragma unroll
