@@ -173,19 +173,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     if (lane < boxes)
                         tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, map, lane % PARTS * 64,
                                     place, cur.kh, page, &full[slot]);
-                    // places of the last V tile behind the last position, in its box, may hold anything:
-                    // they are cleared before anyone reads the tile
-                    const int end = cur.hi - (cur.lo_t + cur.kt + i) * KT_TILE;
-                    if (is_v && kt_fix(a, KT_TILE, end)) {
+                    // places of a V tile that no row of the item sees, in a box some row sees
+                    const int j0 = (cur.lo_t + cur.kt + i) * KT_TILE;
+                    if (is_v && kt_fix(a, KT_TILE, lo, cur.hi, j0)) {
                         ok = kt_wait_warp(&full[slot], (uint32_t)turn & 1u, abort_flag, status);
                         if (!ok) break;
-                        const int rows_z = (end + a.box - 1) / a.box * a.box - end;
-                        for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
-                            const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
-                            *reinterpret_cast<uint4 *>(smem + 2 * QT + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_async_smem();
-                        __syncwarp();
+                        kt_clear<KT_TILE, PARTS>(a, smem + 2 * QT + slot * UNIT, lo, cur.hi, j0, lane);
                         if (lane == 0) mbar_arrive(&fixed[slot]);
                     }
                     slot += 2;
@@ -245,7 +238,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     if (!begin(u)) break;
                     const KtRows rt(a, cur, Q, x);
                     const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                    const int first = (cur.lo_t + cur.kt) * KT_TILE;
+                    const int first = (cur.lo_t + cur.kt) * KT_TILE, lo = cur.lo_of(a, cur.pair * Q);
                     if (!wait(&q_full, qp)) break;
                     qp ^= 1;
                     bool begun = false;
@@ -254,7 +247,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                         const int j0 = first + i * KT_TILE;
                         if (i + 1 < n_here) ok = qk(rt.sees(j0 + KT_TILE), i + 2 == n_here);
                         ok = ok && wait(&full[vs], vp);
-                        if (ok && i + 1 == n_here && kt_fix(a, KT_TILE, cur.hi - j0)) {
+                        if (ok && kt_fix(a, KT_TILE, lo, cur.hi, j0)) {
                             ok = wait(&fixed[vs], fp >> vs & 1u);
                             fp ^= 1u << vs;
                         }

@@ -184,8 +184,27 @@ __device__ __forceinline__ bool kt_wait_warp(uint64_t *bar, uint32_t parity, vol
     return __all_sync(0xffffffffu, kt_wait(bar, parity, abort_flag, status));
 }
 
-// Whether a V tile with `end` places up to the item's last position has more in that one's box.
-__device__ __forceinline__ bool kt_fix(const AttendArgs &a, int tile, int end) { return end < tile && end % a.box; }
+// Whether the V tile at position j0 of an item that sees [lo, hi) has places outside that range in the
+// boxes of its first or last position: what they hold is nobody's, and a weight of zero does not silence
+// a NaN, so they are cleared (kt_clear) before the tile is multiplied. (box is a power of two.)
+__device__ __forceinline__ bool kt_fix(const AttendArgs &a, int tile, int lo, int hi, int j0) {
+    return (lo > j0 && (lo - j0) & (a.box - 1)) || (hi < j0 + tile && (hi - j0) & (a.box - 1));
+}
+// Those places become zeros, by one warp, in a tile of PARTS columns of 128 bytes a place.
+template <int TILE, int PARTS>
+__device__ __forceinline__ void kt_clear(const AttendArgs &a, uint8_t *at, int lo, int hi, int j0, int lane) {
+    auto clear = [&](int from, int to) {                  // places [from, to) of the tile
+        for (int z = lane; z < (to - from) * 8 * PARTS; z += 32) {
+            const int row = from + z / (8 * PARTS), c = z % (8 * PARTS);
+            *reinterpret_cast<uint4 *>(at + c / 8 * (TILE * 128) + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+        }
+    };
+    const int front = lo - j0, end = hi - j0;
+    if (front > 0) clear(front & -a.box, front);
+    if (end < TILE) clear(end, (end + a.box - 1) & -a.box);
+    fence_async_smem();
+    __syncwarp();
+}
 
 // Two f32 in one 64-bit register, worked on by one instruction (sm_100).
 typedef unsigned long long f32x2;

@@ -146,18 +146,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                         if (lane < boxes)
                             tma_load_4d(ring + slot * UNIT + lane % PARTS * COL + lane / PARTS * a.box * 128, half ? &tm_v : &tm_k,
                                         lane % PARTS * (128 / ES), place, cur.kh, page, &full[slot]);
-                        // 16-bit cache: clear the places behind the last position (kv_attend_tc.cu)
-                        const int end = cur.hi - (cur.lo_t + cur.kt + i) * KF_TILE;
-                        if (!F32C && half && kt_fix(a, KF_TILE, end)) {
+                        // 16-bit cache: places that no row of the item sees, in a box some row sees
+                        const int j0 = (cur.lo_t + cur.kt + i) * KF_TILE;
+                        if (!F32C && half && kt_fix(a, KF_TILE, lo, cur.hi, j0)) {
                             ok = kt_wait_warp(&full[slot], (uint32_t)turn & 1u, abort_flag, status);
                             if (!ok) break;
-                            const int rows_z = (end + a.box - 1) / a.box * a.box - end;
-                            for (int z = lane; z < rows_z * 8 * PARTS; z += 32) {
-                                const int row = end + z / (8 * PARTS), c = z % (8 * PARTS);
-                                *reinterpret_cast<uint4 *>(smem + slot * UNIT + c / 8 * COL + row * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_async_smem();
-                            __syncwarp();
+                            kt_clear<KF_TILE, PARTS>(a, smem + slot * UNIT, lo, cur.hi, j0, lane);
                             if (lane == 0) mbar_arrive(&fixed[slot]);
                         }
                         slot += 3 - halves;
@@ -216,7 +210,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                 for (long u = u0; u < u1 && ok;) {
                     if (!begin(u)) break;
                     const int n_here = (int)min((long)(cur.nt - cur.kt), u1 - u);
-                    const int first = (cur.lo_t + cur.kt) * KF_TILE;
+                    const int first = (cur.lo_t + cur.kt) * KF_TILE, lo = cur.lo_of(a, cur.pair * TT);
                     if (!wait(&q_full, qp)) break;
                     qp ^= 1;
                     tc_fence_after();
@@ -227,7 +221,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                         ok = ok && wait(&p_full, pp);
                         pp ^= 1;
                         ok = ok && wait(F32C ? &v_full : &full[vs], vp);
-                        if (ok && !F32C && kt_fix(a, KF_TILE, cur.hi - (first + i * KF_TILE))) {
+                        if (ok && !F32C && kt_fix(a, KF_TILE, lo, cur.hi, first + i * KF_TILE)) {
                             ok = wait(&fixed[vs], fp >> vs & 1u);
                             fp ^= 1u << vs;
                         }

@@ -333,6 +333,31 @@ def test_pages_in_front_of_the_window_may_be_gone(rt, ct, new):
 
 
 @pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_places_in_front_of_the_window_may_hold_anything(rt, ct, new, page, hd):
+    """A caller that writes only the positions some row sees: every place in front of the first row's
+    window holds NaN and infinities, those of a page that is still read among them."""
+    from cachepotato_b200.kv import KVCache
+    for window in (1, 33, 70):
+        b = R.Batch([(new, 500), (new, 3), (new, 117)], page, 6)
+        kp, vp = R.pools(b, 2, hd, TYPES[ct], 7)
+        q = rows((b.rows, 8, hd), TYPES[rt], 8)
+        want, size = R.attend(b, q, kp, vp, hd ** -0.5, window)
+        tol = attend_tol(b, want, size, vp, TYPES[rt])
+        for i, (_, c) in enumerate(b.lens):
+            at = b.place(i, torch.arange(max(0, c - window + 1)))
+            page_at, place = (x.cuda() for x in at)
+            kp[page_at, place] = float("nan")
+            vp[page_at, place] = torch.tensor([float("inf"), float("nan"), -float("inf"), float("nan")], dtype=TYPES[ct],
+                                              device="cuda").repeat(hd // 4)
+        cache = KVCache(kp, vp, rope_dim=0)
+        close(cache.attend(b.device(new), q, window=window), want, tol, f"window {window}")
+        cache.check()
+
+
+@pytest.mark.parametrize("rt,ct", COMBOS)
 def test_one_pool_for_keys_and_values(rt, ct):
     """Keys and values side by side in one tensor, part of a wider one: strides of no dense layout."""
     from cachepotato_b200.kv import KVCache
