@@ -126,19 +126,16 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
         const int t = t0 + r, i = kv_find_seq(a.b.q_start, a.b.n, t);
         int pos = -1, page = -1;
         if (i < a.b.n) {
-            const int a0 = a.b.q_start[i], p0 = a.b.pos0[i];
-            if (t >= a0 && p0 >= 0) {
-                const long p = (long)p0 + (t - a0);
-                pos = (int)min(p, 0x7fffffffl);
-                const int at = pos / a.c.P;
-                const bool inside = p < 0x7fff0000l && at < a.b.max_pages;
-                if (inside) page = a.b.pages[(size_t)i * a.b.table_stride + at];
-                if (page < 0 || page >= a.c.n_pages) {
-                    page = -1;
-                    if (lane == 0) atomicOr(a.c.status, inside ? KV_BAD_PAGE : KV_BAD_POS);
+            const KvSeq q = kv_seq(a.b, a.c.P, i);
+            if (q.r0 >= 0 && t >= q.r0 && q.p0 >= 0) {
+                pos = (int)min((long)q.p0 + (t - q.r0), 0x7fffffffl);
+                if (t - q.r0 < q.len) {                   // (its place is in the table)
+                    page = a.b.pages[(size_t)i * a.b.table_stride + pos / a.c.P];
+                    if (page < 0 || page >= a.c.n_pages) {
+                        page = -1;
+                        if (lane == 0) atomicOr(a.c.status, KV_BAD_PAGE);
+                    }
                 }
-            } else if (lane == 0 && p0 < 0) {
-                atomicOr(a.c.status, KV_BAD_POS);
             }
         }
         if (lane == 0) {
@@ -249,6 +246,9 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
             load_kv(xkv, t, h);
         }
     }
+    // every sequence is looked at once, whether a row led to it or not
+    for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + tid; i < a.b.n; i += (size_t)gridDim.x * gridDim.y * blockDim.x)
+        if (kv_seq(a.b, a.c.P, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
 }
 
 template <typename TI, typename TC>

@@ -78,7 +78,8 @@ __device__ __forceinline__ int kv_find_seq(const int *__restrict__ q_start, int 
 }
 
 // Sequence i's rows [r0, r0 + len) and the position of its first one, made safe: rows inside
-// [0, T), positions inside the table (rows past it are cut off). bad: something had to be cut.
+// [0, T), positions inside the table (rows past either are cut off, and a sequence whose start or
+// first position is negative, or that ends before it starts, has none). bad: something of it was cut.
 struct KvSeq {
     int r0, len, p0;
     bool bad;
@@ -86,15 +87,15 @@ struct KvSeq {
 __device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int P, int i) {
     KvSeq s;
     const int a = b.q_start[i], e = b.q_start[i + 1];
+    s.r0 = a;
     s.p0 = b.pos0[i];
-    s.r0 = max(a, 0);
-    s.len = max(0, min(e, b.T) - s.r0);
-    s.bad = a < 0 || e < a || e > b.T || s.p0 < 0;
-    const long cap = min((long)b.max_pages * P, 0x7fff0000l);   // positions and tile ends stay in 32 bits
-    if (s.p0 < 0) s.len = 0;
-    if ((long)s.p0 + s.len > cap) {
-        s.len = (int)max(0l, cap - s.p0);
-        s.bad = true;
+    s.len = 0;
+    s.bad = a < 0 || e < a || e > b.T || (e > a && s.p0 < 0);    // (no rows: pos0 may be anything)
+    if (a >= 0 && s.p0 >= 0 && min(e, b.T) > a) {
+        const long cap = min((long)b.max_pages * P, 0x7fff0000l);   // positions and tile ends stay in 32 bits
+        const int n = min(e, b.T) - a;
+        s.len = (int)min((long)n, max(0l, cap - s.p0));
+        s.bad = s.bad || s.len < n;
     }
     return s;
 }

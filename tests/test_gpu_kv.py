@@ -454,6 +454,74 @@ def test_attend_bad_tables_touch_nothing():
             cache.check()
 
 
+def bad_starts(good, T):
+    """Starts no batch has, each with what is wrong about it."""
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    made = []
+    for at, values in ((0, (lo, -1, hi)), (1, (lo, -7, hi, T + 1)), (2, (lo, 0, hi, T + 9)), (3, (lo, 0, 1, hi, T + 1))):
+        for v in values:
+            s = good.copy()
+            s[at] = v
+            made.append(s)
+    return made + [good[::-1].copy(), np.full_like(good, lo), np.full_like(good, hi), np.array([hi, lo, hi, lo], np.int32)]
+
+
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 90])
+def test_bad_starts_are_reported_and_touch_nothing(rt, ct, new):
+    """Negative, descending and too large starts: both operators report them, once, and write nothing
+    outside the rows, or outside the pages of the table; the next call is right."""
+    from cachepotato_b200 import CpgError
+    from cachepotato_b200.kv import KVBatch, KVCache
+    H, KV, hd, page, guard = 8, 2, 64, 16, 8
+    b = R.Batch([(1, 50), (new, 50), (2, 130)], page, 6, spare=9)
+    kp, vp = R.pools(b, KV, hd, TYPES[ct], 7)
+    T = b.rows
+    free = torch.ones(b.n_pages, dtype=torch.bool, device="cuda")
+    free[torch.from_numpy(b.table[b.table >= 0]).long().cuda()] = False
+    qkv = rows((T + 2 * guard, H + 2 * KV, hd), TYPES[rt], 8)
+    q, k, v = (qkv[guard:guard + T, x] for x in (slice(0, H), slice(H, H + KV), slice(H + KV, None)))
+    cache = KVCache(kp, vp)
+    good = b.device(new)
+    ws = cache.workspace(H)
+    out = torch.full((T + 2 * guard, H, hd), 7.0, dtype=TYPES[rt], device="cuda")
+    inner = out[guard:guard + T]
+    want_q = cache.append(good, q, k, v).clone()
+    want = cache.attend(good, want_q, ws=ws)
+    kept = [p.clone() for p in (kp, vp)]
+    cache.check()
+    for s in bad_starts(b.start, T):
+        bad = KVBatch(torch.from_numpy(s).cuda(), good.pos0, good.pages, rows=T, max_new=new)
+        for call in (lambda: cache.append(bad, q, k, v, q_out=inner), lambda: cache.attend(bad, want_q, out=inner, ws=ws)):
+            call()
+            with pytest.raises(CpgError):
+                cache.check()
+            cache.check()
+            assert bool((out[:guard] == 7.0).all()) and bool((out[guard + T:] == 7.0).all()), s
+            assert all(torch.equal(p[free], x[free]) for p, x in zip((kp, vp), kept)), s
+        for p, x in zip((kp, vp), kept):
+            p.copy_(x)
+        assert torch.equal(cache.append(good, q, k, v), want_q) and torch.equal(cache.attend(good, want_q, ws=ws), want), s
+        assert all(torch.equal(p, x) for p, x in zip((kp, vp), kept))
+        cache.check()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_sequence_without_rows_may_stand_anywhere(new):
+    """A padded batch: the position and the pages of a sequence that brings no rows are not looked at."""
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(0, 5), (new, 50), (0, 9), (1, 130), (0, 0)], 16, 6)
+    kp, vp = R.pools(b, 2, 64, torch.bfloat16, 7)
+    q, k = rows((b.rows, 8, 64), torch.bfloat16, 8), rows((b.rows, 2, 64), torch.bfloat16, 9)
+    cache, batch = KVCache(kp, vp), b.device(new)
+    made = cache.append(batch, q, k, k)
+    want = cache.attend(batch, made)
+    batch.pos0[torch.tensor([0, 2, 4], device="cuda")] = torch.tensor([-1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    batch.pages[torch.tensor([0, 2, 4], device="cuda")] = -1
+    assert torch.equal(cache.append(batch, q, k, k), made) and torch.equal(cache.attend(batch, made), want)
+    cache.check()
+
+
 def test_empty_batches():
     from cachepotato_b200.kv import KVCache
     b = R.Batch([(0, 5), (0, 0)], 16, 1, pad=4)
