@@ -231,7 +231,11 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
     };
     if (n > KD_THREADS) {                                 // more sequences than threads: their sum first
         long sum = 0;
-        for (int i = tid; i < n; i += KD_THREADS) sum += kd_seq<ROWS>(a, G, i).units;
+        for (int i = tid; i < n; i += KD_THREADS) {
+            const KdSeq q = kd_seq<ROWS>(a, G, i);
+            sum += q.units;
+            if (q.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_scan[warp] = sum;
@@ -247,7 +251,8 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
         if (c0 + tid < n) {
             mine = kd_seq<ROWS>(a, G, c0 + tid);
             inc = mine.units;
-            if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
+            // (of more, all have been looked at above: this loop ends at the block's own)
+            if (n <= KD_THREADS && mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
         }
         const long x = inc;
 #pragma unroll

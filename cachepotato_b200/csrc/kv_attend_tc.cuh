@@ -96,7 +96,11 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
     };
     if (n > KT_THREADS) {                                 // more sequences than threads: their sum first
         long sum = 0;
-        for (int i = tid; i < n; i += KT_THREADS) sum += kt_seq<TILE, FIXED>(a, Q, i).head_units * a.c.KV;
+        for (int i = tid; i < n; i += KT_THREADS) {
+            const KtSeq q = kt_seq<TILE, FIXED>(a, Q, i);
+            sum += q.head_units * a.c.KV;
+            if (q.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) sh.scan[warp] = sum;
@@ -110,7 +114,8 @@ __device__ __forceinline__ bool kt_begin(const AttendArgs &a, int Q, KtShared<TI
         KtSeq mine{};
         if (c0 + tid < n) {
             mine = kt_seq<TILE, FIXED>(a, Q, c0 + tid);
-            if (mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
+            // (of more, all have been looked at above: this loop ends at the block's own)
+            if (n <= KT_THREADS && mine.s.bad && blk == 0) atomicOr(a.c.status, KV_BAD_POS);
         }
         const long x = mine.head_units * a.c.KV;
         long inc = x;

@@ -522,6 +522,36 @@ def test_a_sequence_without_rows_may_stand_anywhere(new):
     cache.check()
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("n", [3, 160, 170, 384, 400])
+@pytest.mark.parametrize("chunk", [1, 40])
+def test_every_bad_sequence_is_reported(rt, ct, n, chunk):
+    """More sequences than a block has threads: the last one past its table, and all of them."""
+    from cachepotato_b200 import CpgError
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(chunk, 9)] + [(1, 5)] * (n - 1), 8, 6, wide=0)
+    kp, vp = R.pools(b, 2, 64, TYPES[ct], 7)
+    q, k = rows((b.rows, 8, 64), TYPES[rt], 8), rows((b.rows, 2, 64), TYPES[rt], 9)
+    cache, batch = KVCache(kp, vp, rope_dim=0), b.device(chunk)
+    ws = cache.workspace(8)
+    calls = [lambda: cache.append(batch, q, k, k), lambda: cache.attend(batch, q, ws=ws)]
+    want = [call() for call in calls]
+    cache.check()
+    pos0 = batch.pos0.clone()
+    wide = b.table.shape[1] * 8
+    for places in (slice(n - 1, n), slice(0, n)):
+        for bad in (wide, 2 ** 31 - 40, -3):                      # one past the table, far past, in front
+            batch.pos0[places] = bad
+            for call in calls:
+                call()
+                with pytest.raises(CpgError):
+                    cache.check()
+                cache.check()
+            batch.pos0.copy_(pos0)
+    assert all(torch.equal(call(), w) for call, w in zip(calls, want))
+    cache.check()
+
+
 def test_empty_batches():
     from cachepotato_b200.kv import KVCache
     b = R.Batch([(0, 5), (0, 0)], 16, 1, pad=4)
