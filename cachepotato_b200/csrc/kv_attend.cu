@@ -573,7 +573,8 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                         float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float mn = fmaxf(m[r], mx * sc[r]), base = mn == -INFINITY ? 0.0f : mn;
+                        const float mn = fmaxf(m[r], kv_top<HALF>(mx * sc[r])), base = mn == -INFINITY ? 0.0f : mn;
+                        const float minus = kv_lift<HALF>(14.0f) - base;
                         c[r] = ex2(m[r] - base);
                         m[r] = mn;
                         float add = 0.0f;
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
                             for (int e = 2 * r; e < 2 * r + 2; ++e) {
-                                s[n][e] = ex2(fmaf(s[n][e], sc[r], -base));
+                                s[n][e] = ex2(fmaf(s[n][e], sc[r], minus));
                                 add += s[n][e];
                             }
                         l[r] = fmaf(l[r], c[r], add);

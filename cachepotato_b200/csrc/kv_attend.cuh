@@ -26,6 +26,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Weights that go into f16 operands are lifted by 2^14 (kv_attend_tc.cu, which lets them grow to 2^8 before
+// it rescales: by 2^7): f16 has nothing below 2^-25, and of a long cache thousands of weights of 2^-26 of
+// the largest one count. l and o carry the factor, which cancels in o / l. So that it can be taken off the
+// maximum exactly, an f16 cache's running maxima are rounded up to whole numbers (in powers of two).
+template <bool HALF> __device__ __forceinline__ float kv_top(float top) { return HALF ? ceilf(top) : top; }
+template <bool HALF> constexpr float kv_lift(float by) { return HALF ? by : 0.0f; }
+
 // (x, y) as N terms of two 16-bit halves each, largest first. f16: rounded, 22 bits from two terms.
 // bf16: one term rounded; three terms cut off, which leaves nothing of an f32.
 template <bool HALF, int N>

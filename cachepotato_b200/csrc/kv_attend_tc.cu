@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
 #pragma unroll
                 for (int e = 0; e < KT_TILE; e += 2)
                     mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+                const float top = kv_top<HALF>(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2);
                 const bool grow = top > m + 8.0f;
                 if (__any_sync(0xffffffffu, grow)) {      // O and l to the scale of a larger maximum
                     const float f = grow ? ex2(m - top) : 1.0f;
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tc(const __grid_con
                     }
                 }
                 begun = true;
-                const float base = m == -INFINITY ? 0.0f : m;
-                const f32x2 minus = pack2(-base, -base), scale22 = pack2(a.scale2, a.scale2);
+                const float off = kv_lift<HALF>(7.0f) - (m == -INFINITY ? 0.0f : m);
+                const f32x2 minus = pack2(off, off), scale22 = pack2(a.scale2, a.scale2);
                 f32x2 add[2] = {0, 0};
 #pragma unroll
                 for (int e = 0; e < KT_TILE / 2; ++e) {   // the weights, packed into the registers behind

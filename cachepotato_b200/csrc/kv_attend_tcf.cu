@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int e = 0; e < 64; e += 2) mx[e / 2 & 3] = fmaxf(mx[e / 2 & 3], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc), base = mn == -INFINITY ? 0.0f : mn;
+                const float mn = fmaxf(m, kv_top<HALF>(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc));
+                const float base = mn == -INFINITY ? 0.0f : mn, minus = kv_lift<HALF>(14.0f) - base;
                 f = ex2(m - base);
                 m = mn;
                 float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -412,8 +413,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                     uint32_t w[NQ][8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float e0 = ex2(fmaf(__uint_as_float(s[16 * c + 2 * e]), sc, -base));
-                        const float e1 = ex2(fmaf(__uint_as_float(s[16 * c + 2 * e + 1]), sc, -base));
+                        const float e0 = ex2(fmaf(__uint_as_float(s[16 * c + 2 * e]), sc, minus));
+                        const float e1 = ex2(fmaf(__uint_as_float(s[16 * c + 2 * e + 1]), sc, minus));
                         add[e & 1] += e0;
                         add[2 + (e & 1)] += e1;
                         uint32_t t[NQ];

@@ -304,6 +304,37 @@ def test_attend_scores_of_any_size(rt, ct):
         close(got, want, attend_tol(b, want, size, vp, TYPES[rt]), kind)
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 40])
+def test_attend_many_small_weights(rt, ct, new):
+    """A few keys at the start outweigh each of the others by far, and all of them together not at all:
+    thousands of equal weights of 2^-15 to 2^-26 of the largest. Values are positive, so what each weight is
+    off by adds up, and is relative to the result: attend_tol's parts, a half step of a 16-bit weight (and one of the result), and
+    2^-25 of a lifted f16 one, the largest of which is over 2^6 (so 2^-31 each). 300 sequences over the same pages: a block then works through most of one, with the
+    large keys in front, where a lone sequence would be spread over all blocks."""
+    from cachepotato_b200.kv import KVBatch, KVCache
+    hd, H, S = 64, 4, 300
+    for n, below in ((4000, 10.5), (4000, 17.4), (131000, 10.0), (131000, 14.1), (131000, 17.4), (131000, 18.0)):
+        b = R.Batch([(new, n)], 256, 8)
+        kp, vp = R.pools(b, 1, hd, TYPES[ct], 9)
+        vp.copy_((1 + 0.1 * vp.float()).to(TYPES[ct]))
+        q = torch.zeros((new, H, hd), dtype=TYPES[rt], device="cuda")
+        q[..., 0] = 8.0
+        kp.zero_()
+        page, at = (x.cuda() for x in b.place(0, torch.arange(0, 64, 16)))
+        kp[page, at, 0, 0] = below                                # a score of `below`; the others' are 0
+        vp[page, at] = 0.25
+        want, size = R.attend(b, q, kp, vp, hd ** -0.5, 0)
+        tol = (2 * (16 * size + 4) + (n + new) / 16 + 32) * U * want
+        if rt != "f32":
+            tol = tol + half_step(TYPES[rt]) * 2 * want * (1 + 2 ** -7) + n * 2.0 ** -31 * vp.max().double()
+        i32 = dict(dtype=torch.int32, device="cuda")
+        batch = KVBatch(torch.arange(S + 1, **i32) * new, torch.full((S,), n, **i32),
+                        torch.from_numpy(b.table).cuda().repeat(S, 1), rows=S * new, max_new=new)
+        got = KVCache(kp, vp, rope_dim=0).attend(batch, q.repeat(S, 1, 1))
+        close(got, want.repeat(S, 1, 1), tol.expand(want.shape).repeat(S, 1, 1), f"{n}, {below}")
+
+
 def test_attend_scale_and_in_place():
     from cachepotato_b200.kv import KVCache
     for rt, ct in COMBOS:
