@@ -35,7 +35,8 @@
 //           rest the joins of 74 parts); one f32 row over 512 positions: 11 us.
 //   types   16-bit rows: one product per step, P rounded to the cache's type (its rounding is as
 //           large as the result's own). f32 rows keep about 22 bits: over an f16 cache q (scaled by
-//           a power of two per row) and P are split into two f16 terms; over a bf16 cache into three
+//           a power of two per row, as far up as f16 goes: the small elements of a row with a large one
+//           keep their bits) and P are split into two f16 terms; over a bf16 cache into three
 //           bf16 terms; over an f32 cache K and V are split as well (three bf16 terms by truncation,
 //           exact) and the six products of weight 2^-16 and more are kept. The tensor core cuts
 //           off what it adds to an accumulator instead of rounding, so for f32 rows an accumulator
@@ -434,12 +435,12 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                         }
                         mx = fmaxf(mx, fmaxf(fmaxf(fabsf(f[r][ks][0]), fabsf(f[r][ks][1])), fmaxf(fabsf(f[r][ks][2]), fabsf(f[r][ks][3]))));
                     }
-                    if constexpr (HALF) {                 // the row into f16's range by a power of two
+                    if constexpr (HALF) {                 // the row by a power of two so that its largest is in [2^14, 2^15)
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const int eb = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
-                        up[r] = __uint_as_float((uint32_t)(254 - eb) << 23);
-                        sc[r] = a.scale2 * __uint_as_float((uint32_t)eb << 23);
+                        const int eb = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
+                        up[r] = __uint_as_float((uint32_t)(268 - eb) << 23);
+                        sc[r] = a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23);
                     }
                 }
                 m[r] = -INFINITY;

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
             {                                             // q's terms
                 const float4 *const src = (const float4 *)((const float *)a.q + cell * a.q_stride + (size_t)(cur.kh * G + g) * HD);
                 float up = 1.0f;
-                if constexpr (HALF) {                     // the row into f16's range by a power of two
+                if constexpr (HALF) {                     // the row by a power of two so that its largest is in [2^14, 2^15)
                     float mx = 0.0f;
                     if (live) {
 #pragma unroll 8
@@ -332,9 +332,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                             mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
                         }
                     }
-                    const int eb = min(max((int)(__float_as_uint(mx) >> 23), 1), 253);
-                    up = __uint_as_float((uint32_t)(254 - eb) << 23);
-                    sc = a.scale2 * __uint_as_float((uint32_t)eb << 23);
+                    const int eb = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
+                    up = __uint_as_float((uint32_t)(268 - eb) << 23);
+                    sc = a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23);
                 }
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {

@@ -335,6 +335,27 @@ def test_attend_many_small_weights(rt, ct, new):
         close(got, want.repeat(S, 1, 1), tol.expand(want.shape).repeat(S, 1, 1), f"{n}, {below}")
 
 
+@pytest.mark.parametrize("rt,ct", [c for c in COMBOS if c[0] == "f32"])
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_rows_with_one_large_element(rt, ct, new, hd):
+    """f32 rows keep their precision beside an element that is 30000 times as large and meets zeros."""
+    from cachepotato_b200.kv import KVCache
+    for big in (30000.0, -1.2e-30, 0.0):                          # the rest is scaled like it: 1, 4e-35, and plain
+        b = R.Batch([(new, 20), (new, 3)], 16, 8)
+        kp, vp = R.pools(b, 1, hd, TYPES[ct], 9)
+        q = rows((b.rows, 8, hd), torch.float32, 10)
+        scale = hd ** -0.5
+        if big:
+            kp[..., 5] = 0.0
+            q.mul_(abs(big) / 30000)
+            scale *= 30000 / abs(big)
+            q[..., 5] = big
+        want, size = R.attend(b, q, kp, vp, scale, 0)
+        got = KVCache(kp, vp, rope_dim=0).attend(b.device(new), q, scale=scale)
+        close(got, want, attend_tol(b, want, size, vp, torch.float32), f"{big}")
+
+
 def test_attend_scale_and_in_place():
     from cachepotato_b200.kv import KVCache
     for rt, ct in COMBOS:
