@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(KD_THREADS, 2) k_kv_attend(const __grid_consta
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                         const int eb = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
                         up[r] = __uint_as_float((uint32_t)(268 - eb) << 23);
-                        sc[r] = a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23);
+                        sc[r] = fmaxf(a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23), 0x1p-126f);   // (a zero would make hidden scores NaN)
                     }
                 }
                 m[r] = -INFINITY;

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv_attend_tcf(const __grid_co
                     }
                     const int eb = min(max((int)(__float_as_uint(mx) >> 23), 15), 254);
                     up = __uint_as_float((uint32_t)(268 - eb) << 23);
-                    sc = a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23);
+                    sc = fmaxf(a.scale2 * __uint_as_float((uint32_t)(eb - 14) << 23), 0x1p-126f);   // (a zero would make hidden scores NaN)
                 }
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {

@@ -356,6 +356,21 @@ def test_attend_rows_with_one_large_element(rt, ct, new, hd):
         close(got, want, attend_tol(b, want, size, vp, torch.float32), f"{big}")
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 90])
+def test_attend_rows_of_zeros_and_small_scales(rt, ct, new):
+    """Rows of zeros among others, and a scale that makes all weights equal."""
+    from cachepotato_b200.kv import KVCache
+    for scale in (0.125, 1e-9, 1e-37):
+        b = R.Batch([(new, 20), (new, 3)], 16, 8)
+        kp, vp = R.pools(b, 1, 64, TYPES[ct], 9)
+        q = rows((b.rows, 8, 64), TYPES[rt], 10)
+        q[::2] = 0.0
+        want, size = R.attend(b, q, kp, vp, scale, 0)
+        got = KVCache(kp, vp, rope_dim=0).attend(b.device(new), q, scale=scale)
+        close(got, want, attend_tol(b, want, size, vp, TYPES[rt]), f"scale {scale}")
+
+
 def test_attend_scale_and_in_place():
     from cachepotato_b200.kv import KVCache
     for rt, ct in COMBOS:
