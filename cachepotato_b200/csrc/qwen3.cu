@@ -1815,8 +1815,15 @@ static int paged_run(cpg_qwen3_paged *p, const QwPaged &pg, int n, int n_steps) 
     return CPG_OK;
 }
 
-static int paged_status(cpg_qwen3_paged *p, const char *fn) {
-    const int rc = cpg_kv_check(p->kv[0], p->m->s);
+// The end of a step whose launches gave `rc`: n ids to the host, and what its kernels have reported.
+// After an error the caller moves no position, so the step can be repeated, and the stream is idle: the
+// next call writes the pinned arrays that this one's copies read.
+static int paged_finish(cpg_qwen3_paged *p, int rc, int *to, const int *from, size_t n, const char *fn) {
+    cudaError_t ce = cudaSuccess;
+    if (!rc) ce = cudaMemcpyAsync(to, from, sizeof(int) * n, cudaMemcpyDeviceToHost, p->m->s);
+    const cudaError_t se = cudaStreamSynchronize(p->m->s);
+    if (!rc && (ce != cudaSuccess || se != cudaSuccess)) rc = cuda_fail(ce != cudaSuccess ? ce : se, fn);
+    if (!rc) rc = cpg_kv_check(p->kv[0], p->m->s);
     return rc ? rc : qwen3_status(p->m, fn);
 }
 
@@ -1837,21 +1844,15 @@ extern "C" int cpg_qwen3_paged_step(cpg_qwen3_paged *p, const int *slots, const 
     if (rc) return rc;
     QwPaged pg;
     rc = paged_upload(p, slots, n_new, ids, n, (int)T, &pg);
+    if (!rc) rc = T == n ? paged_run(p, pg, n, 1) : qwen3_enqueue(m, paged_seq(p, &pg), (int)T, m->s);
+    rc = paged_finish(p, rc, p->h_out, p->d_next, n, fn);
     if (rc) return rc;
-    if (T == n) {
-        rc = paged_run(p, pg, n, 1);
-    } else {
-        rc = qwen3_enqueue(m, paged_seq(p, &pg), (int)T, m->s);
-    }
-    if (rc) return rc;
-    CPG_CUDA(cudaMemcpyAsync(p->h_out, p->d_next, sizeof(int) * n, cudaMemcpyDeviceToHost, m->s));
-    CPG_CUDA(cudaStreamSynchronize(m->s));
     for (int i = 0; i < n; ++i) {
         p->pos[slots[i]] = std::max(p->pos[slots[i]], 0) + n_new[i];
         next_ids[i] = p->h_out[i];
     }
     p->last_rows = n;
-    return paged_status(p, fn);
+    return CPG_OK;
 }
 
 extern "C" int cpg_qwen3_paged_generate(cpg_qwen3_paged *p, const int *slots, const int *ids, int n, int n_steps, int *out_ids) {
@@ -1866,12 +1867,11 @@ extern "C" int cpg_qwen3_paged_generate(cpg_qwen3_paged *p, const int *slots, co
     QwPaged pg;
     rc = paged_upload(p, slots, nullptr, ids, n, n, &pg);
     if (!rc) rc = paged_run(p, pg, n, n_steps);
+    rc = paged_finish(p, rc, out_ids, p->d_out, (size_t)n * n_steps, fn);
     if (rc) return rc;
-    CPG_CUDA(cudaMemcpyAsync(out_ids, p->d_out, sizeof(int) * (size_t)n * n_steps, cudaMemcpyDeviceToHost, m->s));
-    CPG_CUDA(cudaStreamSynchronize(m->s));
     for (int i = 0; i < n; ++i) p->pos[slots[i]] += n_steps;
     p->last_rows = n;
-    return paged_status(p, fn);
+    return CPG_OK;
 }
 
 extern "C" int cpg_qwen3_paged_drop(cpg_qwen3_paged *p, int slot) {

@@ -220,3 +220,52 @@ def test_pools_no_memory_holds(orc):
         p.close()
     finally:
         gm.close()
+
+
+def _report(p, page, n_pages, max_ctx, bits):
+    """Puts `bits` into the cache's status word, where a kernel whose wait gave up leaves them. (No call
+    hands the word out: it is found through the handles, whose members in front of it are checked.)"""
+    import ctypes
+    from cachepotato_b200.workload import device_view
+    at = lambda where, n, t: [x for x in (t * n).from_address(where)]
+    h = p.handle.value
+    assert at(h + 8, 5, ctypes.c_int) == [p.n_slots, max_ctx, page, -(-max_ctx // page), n_pages]
+    kv = at(at(h + 40, 1, ctypes.c_void_p)[0], 1, ctypes.c_void_p)[0]       # the vector's first handle
+    assert at(kv + 40, 2, ctypes.c_int) == [page, n_pages]
+    word = device_view(torch, at(kv + 56, 1, ctypes.c_void_p)[0], 4, "i4")
+    assert int(word[0]) == 0
+    word.fill_(bits)
+    torch.cuda.synchronize()
+
+
+def test_a_step_that_failed_can_be_repeated(orc):
+    """A step whose kernels report that a wait gave up moves no position: the same call again writes the
+    same places, and the ids are the model's."""
+    from cachepotato_b200 import CpgError, _lib
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    m = _small(orc, 91)
+    a, b = _prompts(m.vocab, [11, 5], 92)
+    gm = device_model(m, max_ctx=64)
+    p = Qwen3Paged(gm, 2, 64, n_pages=16, page_size=8)
+    timeout = 4
+
+    def twice(call, before):
+        rows = tuple(p.logits().shape) if before != (-1, -1) else None
+        _report(p, 8, 16, 64, timeout)
+        with pytest.raises(CpgError) as e:
+            call()
+        assert e.value.code == _lib.CPG_ETIMEOUT
+        assert (p.position(0), p.position(1)) == before
+        assert rows is None or tuple(p.logits().shape) == rows
+        return call()
+    try:
+        x = twice(lambda: p.step([1, 0], [a[:7], b]), (-1, -1))
+        x = twice(lambda: p.step([1], [a[7:]]), (5, 7)).tolist() + x[1:].tolist()        # slots 1, 0
+        y = twice(lambda: p.step([1, 0], [[i] for i in x]), (5, 11)).tolist()
+        z = twice(lambda: p.generate([0, 1], [y[1], y[0]], 3), (6, 12))
+        assert (p.position(0), p.position(1)) == (9, 15) and p.free_pages() == 16 - 2 - 2
+        for prompt, got in ((a, [x[0], y[0]] + z[:, 1].tolist()), (b, [x[1], y[1]] + z[:, 0].tolist())):
+            assert got == gm.generate(prompt, 4).tolist()
+    finally:
+        p.close()
+        gm.close()
