@@ -1666,7 +1666,7 @@ extern "C" int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, in
     }
     p->m = m;
     p->S = n_slots; p->C = max_ctx; p->P = page_size; p->n_pages = n_pages;
-    p->W = (max_ctx + page_size - 1) / page_size;
+    p->W = std::min((max_ctx + page_size - 1) / page_size, n_pages);      // no sequence holds more than the pool
     const size_t in_ints = 3 * S + 1 + S * p->W;
     cudaError_t ce = cudaMalloc(&p->pool, (size_t)m->L * 2 * one);
     if (ce == cudaSuccess) ce = cudaMalloc(&p->d_step_in, in_ints * sizeof(int));

@@ -269,3 +269,24 @@ def test_a_step_that_failed_can_be_repeated(orc):
     finally:
         p.close()
         gm.close()
+
+
+def test_tables_are_no_wider_than_the_pool(orc):
+    """max_ctx bounds positions, not memory: 64 tables of a billion positions over eight pages."""
+    from cachepotato_b200 import CpgError, _lib
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    m = _small(orc, 93)
+    ids = _prompts(m.vocab, [60], 94)[0]
+    gm = device_model(m, max_ctx=64)
+    free = torch.cuda.mem_get_info()[0]
+    p = Qwen3Paged(gm, 64, 1 << 30, n_pages=8, page_size=8)
+    try:
+        assert free - torch.cuda.mem_get_info()[0] < 1 << 29
+        first = p.step([63], [ids])
+        assert [int(first[0])] + p.generate([63], first, 4)[:, 0].tolist() == gm.generate(ids, 4).tolist()
+        with pytest.raises(CpgError) as e:
+            p.step([63], [[1]])
+        assert e.value.code == _lib.CPG_ENOMEM and p.position(63) == 64 and p.free_pages() == 0
+    finally:
+        p.close()
+        gm.close()
