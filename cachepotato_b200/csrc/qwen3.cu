@@ -1706,9 +1706,7 @@ extern "C" int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, in
 }
 
 extern "C" void cpg_qwen3_paged_destroy(cpg_qwen3_paged *p) {
-    if (!p) return;
-    cudaStreamSynchronize(p->m->s);
-    paged_free(p);
+    if (p) paged_free(p);                                // (idle: every call ends with its stream synchronised)
 }
 
 // The named slots: distinct, each with room for its new rows; pages for all of them, or none taken.

@@ -290,3 +290,16 @@ def test_tables_are_no_wider_than_the_pool(orc):
     finally:
         p.close()
         gm.close()
+
+
+def test_the_model_may_be_closed_first(orc):
+    """A pool left over by its model can still be closed, and closed twice."""
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    m = _small(orc, 95)
+    for _ in range(3):
+        gm = device_model(m, max_ctx=64)
+        p = Qwen3Paged(gm, 2, 64, n_pages=8, page_size=16)
+        p.step([0], [[1, 2, 3]])
+        gm.close()
+        p.close()
+        p.close()
