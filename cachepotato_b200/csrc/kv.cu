@@ -338,6 +338,8 @@ static int kv_create(const cpg_kv_desc *d, const cpg_kv *like, cpg_kv **out) {
     if (like) kv->v.status = like->v.status;
     if (ce == cudaSuccess && !like) ce = cudaMalloc(&kv->v.status, sizeof(KvDevice));
     if (ce == cudaSuccess && !like) ce = cudaMemcpy(kv->v.status, &dev, sizeof(KvDevice), cudaMemcpyHostToDevice);
+    // (the copy out of pageable memory may return before it has landed; the caller's stream need not wait for it)
+    if (ce == cudaSuccess && !like) ce = cudaStreamSynchronize(cudaStreamLegacy);
     if (ce != cudaSuccess) {
         if (kv->owns) cudaFree(kv->v.status);
         delete kv;

@@ -718,6 +718,24 @@ def test_outputs_made_for_another_stream():
         cache.append(batch, None, k, k, q_out=q)
 
 
+def test_a_new_cache_on_another_stream():
+    """A stream that does not wait for the default one sees a handle's angles as soon as there is a handle."""
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(40, 300), (1, 5)], 16, 3)
+    kp, vp = R.pools(b, 2, 64, torch.float32, 4)
+    batch = b.device(40)
+    q, k = rows((b.rows, 8, 64), torch.float32, 5), rows((b.rows, 2, 64), torch.float32, 6)
+    made = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    for theta in (1e4, 5e5, 1e6, 77.0):
+        torch.cuda.synchronize()
+        cache = KVCache(kp, vp, rope_theta=theta)
+        cache.append(batch, q, k, k, q_out=made, stream=side)
+        side.synchronize()
+        assert torch.equal(made, cache.append(batch, q, k, k))
+        cache.check()
+
+
 def test_attend_is_the_same_every_time():
     """Work split over blocks is joined in a fixed order."""
     from cachepotato_b200.kv import KVCache
