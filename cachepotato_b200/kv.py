@@ -21,6 +21,9 @@ from ._lib import KvDesc, KvRows, check, lib
 _TYPES = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
 
 
+_ALL = 2 ** 31 - 1                                       # a window past every position (and the C entry's int)
+
+
 def _require(ok: bool, msg: str) -> None:
     if not ok:
         raise _lib.CpgError(_lib.CPG_EINVAL, msg)
@@ -150,11 +153,12 @@ class KVCache:
                 out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         os_ = self._rows(out, "out", batch.rows, heads)
         _require(out.dtype == q.dtype, "out and q must have one type")
+        _require(window >= 0, "window must not be negative")
         if ws is None:
             ws = self.workspace(heads, stream)
         _require(ws.get_device() == self._index and ws.is_contiguous(), "the workspace must be dense, on the cache's device")
         self._call(stream, self._attend, batch._ref, _TYPES[q.dtype], heads, q.data_ptr(), qs, out.data_ptr(), os_,
-                   self._scale if scale is None else scale, window, ws.data_ptr(), ws.numel() * ws.element_size())
+                   self._scale if scale is None else scale, min(window, _ALL), ws.data_ptr(), ws.numel() * ws.element_size())
         return out
 
     def check(self, stream=None) -> None:

@@ -736,6 +736,24 @@ def test_a_new_cache_on_another_stream():
         cache.check()
 
 
+def test_windows_past_every_position():
+    """Windows are whole numbers of any size: one that no int holds is not cut to its low bits."""
+    from cachepotato_b200 import CpgError
+    from cachepotato_b200.kv import KVCache
+    for rt, ct in COMBOS:
+        for new in (1, 90):
+            b = R.Batch([(new, 500), (new, 3)], 16, 8)
+            kp, vp = R.pools(b, 1, 64, TYPES[ct], 9)
+            q = rows((b.rows, 8, 64), TYPES[rt], 10)
+            cache, batch = KVCache(kp, vp, rope_dim=0), b.device(new)
+            want = cache.attend(batch, q)
+            for window in (500 + new, 2 ** 31 - 1, 2 ** 31 + 7, 2 ** 32 + 5, 2 ** 63):
+                assert torch.equal(cache.attend(batch, q, window=window), want), window
+            for window in (-1, -2 ** 31, 5 - 2 ** 32):
+                with pytest.raises(CpgError):
+                    cache.attend(batch, q, window=window)
+
+
 def test_attend_is_the_same_every_time():
     """Work split over blocks is joined in a fixed order."""
     from cachepotato_b200.kv import KVCache
