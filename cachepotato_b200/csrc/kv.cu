@@ -447,7 +447,8 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
                 fn, type, kv->v.type);
     CPG_REQUIRE(n_heads >= 1 && n_heads <= 4096 && n_heads % kv->v.KV == 0, "%s: %d heads over %d cached heads", fn,
                 n_heads, kv->v.KV);
-    CPG_REQUIRE(scale > 0.0f && isfinite(scale), "%s: scale %g must be positive", fn, (double)scale);
+    // (the kernels take it in powers of two)
+    CPG_REQUIRE(scale > 0.0f && isfinite(scale * 1.4426950408889634f), "%s: scale %g must be positive, below 2.3e38", fn, (double)scale);
     CPG_REQUIRE(window >= 0, "%s: window %d", fn, window);
     CPG_REQUIRE((long)r.T * n_heads <= 0x7fff0000l, "%s: %d rows of %d heads", fn, r.T, n_heads);
     if (r.T == 0 || r.n == 0) return CPG_OK;

@@ -754,6 +754,19 @@ def test_windows_past_every_position():
                     cache.attend(batch, q, window=window)
 
 
+def test_scales_too_large_are_refused():
+    """Past 2.3e38 the scale in powers of two leaves f32: such a call would give nothing but NaN."""
+    from cachepotato_b200 import CpgError
+    from cachepotato_b200.kv import KVCache
+    b = R.Batch([(2, 50)], 16, 8)
+    kp, vp = R.pools(b, 1, 64, torch.bfloat16, 9)
+    q = rows((b.rows, 8, 64), torch.bfloat16, 10)
+    cache, batch = KVCache(kp, vp, rope_dim=0), b.device(2)
+    for scale in (3e38, 2.4e38):
+        with pytest.raises(CpgError):
+            cache.attend(batch, q, scale=scale)
+
+
 def test_attend_is_the_same_every_time():
     """Work split over blocks is joined in a fixed order."""
     from cachepotato_b200.kv import KVCache
