@@ -371,6 +371,30 @@ def test_attend_rows_of_zeros_and_small_scales(rt, ct, new):
         close(got, want, attend_tol(b, want, size, vp, TYPES[rt]), f"scale {scale}")
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attend_counts_every_position_once(rt, ct, hd, new):
+    """Equal weights over values that tell which run of 16 positions they come from: each output counts the
+    positions of some runs. Weights and sums are exact, so what remains is the division (4 u) and the
+    result's own rounding; a run lost or added twice is off by some part of a fifth."""
+    from cachepotato_b200.kv import KVCache
+    for window in (0, 1000):
+        b = R.Batch([(new, 5000), (1, 77), (new, 1311), (new, 16 * hd - 1), (0, 4)], 24, 5)
+        kp, vp = R.pools(b, 2, hd, TYPES[ct], 6)
+        vp.zero_()
+        for i, (n, c) in enumerate(b.lens):
+            if n:
+                j = torch.arange(n + c)
+                page, at = b.place(i, j)
+                vp[page.cuda(), at.cuda(), :, (j // 16 % hd).cuda()] = 1.0
+        q = torch.zeros((b.rows, 8, hd), dtype=TYPES[rt], device="cuda")
+        want, _ = R.attend(b, q, kp, vp, hd ** -0.5, window)
+        got = KVCache(kp, vp, rope_dim=0).attend(b.device(new), q, window=window)
+        off = 4 * U if rt == "f32" else half_step(TYPES[rt]) * (1 + 2 ** -7)
+        close(got, want, off * want + tiny(TYPES[rt]), f"window {window}")
+
+
 def test_attend_scale_and_in_place():
     from cachepotato_b200.kv import KVCache
     for rt, ct in COMBOS:

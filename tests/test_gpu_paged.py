@@ -303,3 +303,23 @@ def test_the_model_may_be_closed_first(orc):
         gm.close()
         p.close()
         p.close()
+
+
+def test_more_sequences_than_the_dense_kernels_take(orc):
+    """72 slots: projections and head on the paths for larger steps, prompts and single tokens."""
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    n = 72
+    m = _small(orc, 97)
+    prompts = _prompts(m.vocab, [1 + j % 4 for j in range(n)], 98)
+    gm = device_model(m, max_ctx=256)
+    p = Qwen3Paged(gm, n, 16, n_pages=2 * n, page_size=8)
+    try:
+        first = p.step(np.arange(n), prompts)
+        assert tuple(p.logits().shape) == (n, m.vocab)
+        order = np.random.default_rng(99).permutation(n).astype(np.int32)
+        out = p.generate(order, first[order], 5)
+        for r, j in enumerate(order):
+            assert [int(first[j])] + out[:, r].tolist() == gm.generate(prompts[j], 5).tolist(), j
+    finally:
+        p.close()
+        gm.close()
