@@ -143,6 +143,10 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
             s_page[r] = page;
         }
     }
+    // every sequence is looked at once, whether a row leads to it or not; the last warps first, which
+    // have no row to find where there are few
+    for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x + 1) * blockDim.x - 1 - tid; i < a.b.n; i += (size_t)gridDim.x * gridDim.y * blockDim.x)
+        if (kv_seq(a.b, a.c.P, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
     float gq[2 * E];
     auto gains = [&](const float *g, float *to) {
         get<E>(g + ea, to);
@@ -246,9 +250,6 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
             load_kv(xkv, t, h);
         }
     }
-    // every sequence is looked at once, whether a row led to it or not
-    for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + tid; i < a.b.n; i += (size_t)gridDim.x * gridDim.y * blockDim.x)
-        if (kv_seq(a.b, a.c.P, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
 }
 
 template <typename TI, typename TC>
