@@ -511,6 +511,8 @@ class Qwen3Paged:
         slots = np.ascontiguousarray(slots, dtype=np.int32)
         chunks = [np.atleast_1d(np.asarray(c, dtype=np.int32)) for c in chunks]
         assert len(slots) == len(chunks)
+        if any(c.ndim > 1 for c in chunks):
+            raise _lib.CpgError(_lib.CPG_EINVAL, "Qwen3Paged.step: a chunk is a row of ids, not a table")
         counts = np.array([len(c) for c in chunks], np.int32)
         ids = np.concatenate(chunks) if chunks else np.zeros(0, np.int32)
         out = np.zeros(len(slots), np.int32)

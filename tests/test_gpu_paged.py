@@ -323,3 +323,22 @@ def test_more_sequences_than_the_dense_kernels_take(orc):
     finally:
         p.close()
         gm.close()
+
+
+def test_a_chunk_is_one_row_of_ids(orc):
+    """A table of ids is refused, not cut to the length of its first axis."""
+    from cachepotato_b200 import CpgError
+    from cachepotato_b200.qwen3 import Qwen3Paged
+    m = _small(orc, 101)
+    ids = _prompts(m.vocab, [6], 102)[0]
+    gm = device_model(m, max_ctx=64)
+    p = Qwen3Paged(gm, 2, 32, n_pages=4, page_size=16)
+    try:
+        for chunk in (ids[None], ids[:, None], ids.reshape(2, 3)):
+            with pytest.raises(CpgError):
+                p.step([0], [chunk])
+        assert p.position(0) == -1 and p.free_pages() == 4
+        assert p.step([0], ids[None])[0] == gm.generate(ids, 1)[0]        # (one chunk: the table's row)
+    finally:
+        p.close()
+        gm.close()
