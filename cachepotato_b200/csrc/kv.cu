@@ -48,9 +48,9 @@ namespace cpg {
 // Bound by memory: each value is read and written once. What counts is the bytes in flight, so a
 // thread asks for the next row's heads, unconverted, before it works on this one's, and a run is as
 // long as one wave of blocks needs to take all rows. Measured: 16384 rows of 32 + 2·4 heads in bf16
-// (336 MB) 74 us, 4.5 TB/s (8 bytes a load 85 us; without asking ahead as well 111), in f32 (671 MB)
-// 118 us, 5.7 TB/s (32 bytes a load 162: registers for three blocks instead of four); one row 3.6 us,
-// 64 rows 4.1 us.
+// (336 MB) 75 us, 4.5 TB/s (8 bytes a load 85 us; without asking ahead as well 111), in f32 (671 MB)
+// 117 us, 5.7 TB/s (32 bytes a load 162: registers for three blocks instead of four); in a captured graph
+// one row 3.6 us, 64 rows 4.1 us.
 struct AppendArgs {
     KvRows b;
     KvView c;

@@ -20,8 +20,8 @@
 //           consumer inside an item, and the ring runs on across items. One pass: running maximum
 //           and sum per row in registers, the scores' fragment is the A operand of P·V as it
 //           stands. At an item's end the four warps' (m, l, o) are added in a fixed order.
-//           Places of a page behind what is cached may hold anything: scores there are replaced,
-//           and so are the values' fragments (a weight of zero does not silence a NaN).
+//           Places of a page behind what is cached, or in front of the window, may hold anything: scores
+//           there are replaced, and so are the values' fragments (a weight of zero does not silence a NaN).
 //   join    A block's part of an item that others share goes to the workspace. Parts are joined in
 //           groups of about the root of their number, each by the block that finishes its group last,
 //           and the groups by the one that finishes last of all: two short steps where one block
@@ -29,8 +29,9 @@
 //           is that of the parts, so results do not depend on which block came last.
 //           What counts the parts is one acquire-release addition: a sequentially consistent fence waits
 //           for the tiles in flight, 15 us where a block ends an item in the middle of its range.
-//   measured  128 bf16 rows over 1000-8000 positions (1.14 GB): 188 us, 0.93 of the copy bandwidth; 64 f32
-//           rows over f16, 128-4096 positions (294 MB): 56 us, 0.80; one bf16 row over 128K positions
+//   measured  (on the device, calls in a captured graph) 128 bf16 rows over 1000-8000 positions (1.14 GB):
+//           187 us, 0.93 of the copy bandwidth; 64 f32 rows over f16, 128-4096 positions (294 MB): 56 us,
+//           0.80 (59 from call to call), over bf16 60 us, over f32 (586 MB) 113 us, 0.80; one bf16 row over 128K positions
 //           (268 MB): 59 us, 0.70 (4.5 us until the first tile, 41 of tiles at the copy bandwidth, the
 //           rest the joins of 74 parts); one f32 row over 512 positions: 11 us.
 //   types   16-bit rows: one product per step, P rounded to the cache's type (its rounding is as

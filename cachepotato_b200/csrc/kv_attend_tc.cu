@@ -24,9 +24,11 @@
 //           for two row tiles and 128 positions, of which the tensor core worked half). The tensor core
 //           runs what one thread issues in order, so q·k may overwrite P of the tile before last.
 //   join    Parts of an item that several blocks share, as in kv_attend.cu.
-//   measured  4096 new bf16 rows of 32 heads over 12288 positions and themselves (962 GFLOP): 960 us,
-//           1000 TFLOP/s at the power limit of the GPU (1.7 GHz; 870 us while it is cool); 47 single
-//           rows and a chunk of 2001 over 500-8000 positions (285 GFLOP, 478 MB): 376-400 us; chunks
+//   measured  4096 new bf16 rows of 32 heads over 12288 positions and themselves (962 GFLOP): 865 us while
+//           the GPU is cool, 985 us (980 TFLOP/s) once it is held at its power limit; the tensor pipe and
+//           the exponential unit are each at work in half of the active cycles, so half are lost at any
+//           clock: two softmax warps a scheduler, each with its steps in order. 47 single rows and a chunk
+//           of 2001 over 500-8000 positions (285 GFLOP, 478 MB): 376 us, 425 at the power limit; chunks
 //           with a window of 1000, 14 heads of 64 in f16 (14.6 GFLOP): 50 us.
 #include <math.h>
 

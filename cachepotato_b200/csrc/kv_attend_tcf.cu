@@ -22,7 +22,9 @@
 //   join    Parts of an item that several blocks share, as in kv_attend_tc.cu.
 //   measured  512 f32 rows of 32 heads over themselves, f32 cache (2.1 GFLOP, six times that in bf16
 //           products): 40 us: 2.5 us to the block's range, 4 us for q's terms, 3.3 us a tile (softmax,
-//           p·v and its collection wait for one another), 3.5 us to end an item.
+//           p·v and its collection wait for one another), 3.5 us to end an item; over f16 35 us, bf16 31 us.
+//           2048 rows behind 4096 positions (172 GFLOP): 1186 us over f32, 461 over f16, 537 over bf16.
+//           Heads of 128 spill 128 to 172 bytes a thread.
 #include <math.h>
 
 #include <algorithm>

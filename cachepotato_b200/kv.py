@@ -39,7 +39,9 @@ def _ints(t, what: str, ndim: int, device):
 class KVBatch:
     """The rows of a step: sequence i brings rows q_start[i] .. q_start[i+1]-1, the first of them at
     position pos0[i], its positions in the pages of table row i. The tensors are kept and read when
-    the kernels run: change them in place between steps, or replay a captured step after that."""
+    the kernels run: change them in place between steps, or replay a captured step after that. Rows of
+    no sequence are not written. max_new: the most rows a sequence brings (0: not known), which chooses
+    the kernel: give 1 for a step of single tokens."""
 
     def __init__(self, q_start, pos0, pages, *, rows: int, max_new: int = 0):
         _require(isinstance(q_start, torch.Tensor) and q_start.is_cuda, "q_start must be a CUDA tensor")
@@ -61,7 +63,8 @@ class KVCache:
     """Key and value pools (n_pages, page_size, n_kv, head_dim), f32, f16 or bf16, in any memory order
     whose last axis is dense (a pool stored head by head: pool.transpose(1, 2)). Queries and keys
     are rotated over their first rope_dim elements (None: all of them, 0: none); rope_f32 takes the
-    reference's f32 angles (engine/kernels/kernels.c:425-447) instead of exact ones."""
+    reference's f32 angles (engine/kernels/kernels.c:425-447) instead of exact ones. For inference:
+    results carry no gradient, whatever the inputs ask for."""
 
     def __init__(self, k_pool, v_pool, *, rope_dim: int | None = None, rope_theta: float = 1e6, rope_f32: bool = False):
         for name, p in (("k_pool", k_pool), ("v_pool", v_pool)):
