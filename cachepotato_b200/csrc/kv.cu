@@ -453,6 +453,7 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     CPG_REQUIRE(window >= 0, "%s: window %d", fn, window);
     CPG_REQUIRE((long)r.T * n_heads <= 0x7fff0000l, "%s: %d rows of %d heads", fn, r.T, n_heads);
     if (r.T == 0 || r.n == 0) return CPG_OK;
+    if (window >= (long)r.max_pages * kv->v.P) window = 0;    // hides nothing; the kernels' p - window - j stays in 32 bits
     rc = rows_ok(fn, "q", q, q_stride, n_heads, kv->hd, type);
     if (!rc) rc = rows_ok(fn, "out", out, out_stride, n_heads, kv->hd, type);
     if (rc) return rc;

@@ -778,6 +778,22 @@ def test_windows_past_every_position():
                     cache.attend(batch, q, window=window)
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+def test_windows_as_long_as_the_table(rt, ct):
+    """Windows on both sides of what the table holds give the same rows as none."""
+    from cachepotato_b200.kv import KVCache
+    for new in (1, 90):
+        b = R.Batch([(new, 500), (new, 3)], 16, 8)
+        kp, vp = R.pools(b, 2, 64, TYPES[ct], 9)
+        poison(b, kp, vp)
+        q = rows((b.rows, 8, 64), TYPES[rt], 10)
+        cache, batch = KVCache(kp, vp, rope_dim=0), b.device(new)
+        want, held = cache.attend(batch, q), b.table.shape[1] * 16
+        for window in (500 + new, held - 1, held, held + 1, 2 ** 31 - 1):
+            assert torch.equal(cache.attend(batch, q, window=window), want), window
+        cache.check()
+
+
 def test_scales_too_large_are_refused():
     """Past 2.3e38 the scale in powers of two leaves f32: such a call would give nothing but NaN."""
     from cachepotato_b200 import CpgError
