@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
         const int t = t0 + r, i = kv_find_seq(a.b.q_start, a.b.n, t);
         int pos = -1, page = -1;
         if (i < a.b.n) {
-            const KvSeq q = kv_seq(a.b, a.c.P, i);
+            const KvSeq q = kv_seq(a.b, i);
             if (q.r0 >= 0 && t >= q.r0 && q.p0 >= 0) {
                 pos = (int)min((long)q.p0 + (t - q.r0), 0x7fffffffl);
                 if (t - q.r0 < q.len) {                   // (its place is in the table)
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
     // every sequence is looked at once, whether a row leads to it or not; the last warps first, which
     // have no row to find where there are few
     for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x + 1) * blockDim.x - 1 - tid; i < a.b.n; i += (size_t)gridDim.x * gridDim.y * blockDim.x)
-        if (kv_seq(a.b, a.c.P, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
+        if (kv_seq(a.b, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
     float gq[2 * E];
     auto gains = [&](const float *g, float *to) {
         get<E>(g + ea, to);
@@ -372,7 +372,9 @@ static int kv_rows(const cpg_kv *kv, const cpg_kv_batch *b, const char *fn, KvRo
     int dev = -1;
     CPG_CUDA(cudaGetDevice(&dev));
     CPG_REQUIRE(dev == kv->device, "%s: the cache is on device %d, the current device is %d", fn, kv->device, dev);
-    *r = KvRows{b->n_seqs, b->rows, b->q_start, b->pos0, b->pages, b->table_stride, b->max_pages};
+    // positions and the ends of their tiles stay in 32 bits, and so do a row tile's tiles over all cached heads
+    const long cap = std::min({(long)b->max_pages * kv->v.P, 0x7fff0000l, (1l << 36) / kv->v.KV});
+    *r = KvRows{b->n_seqs, b->rows, b->q_start, b->pos0, b->pages, b->table_stride, (int)cap};
     return CPG_OK;
 }
 
@@ -453,7 +455,7 @@ extern "C" int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, 
     CPG_REQUIRE(window >= 0, "%s: window %d", fn, window);
     CPG_REQUIRE((long)r.T * n_heads <= 0x7fff0000l, "%s: %d rows of %d heads", fn, r.T, n_heads);
     if (r.T == 0 || r.n == 0) return CPG_OK;
-    if (window >= (long)r.max_pages * kv->v.P) window = 0;    // hides nothing; the kernels' p - window - j stays in 32 bits
+    if (window >= r.cap) window = 0;                      // hides nothing; the kernels' p - window - j stays in 32 bits
     rc = rows_ok(fn, "q", q, q_stride, n_heads, kv->hd, type);
     if (!rc) rc = rows_ok(fn, "out", out, out_stride, n_heads, kv->hd, type);
     if (rc) return rc;

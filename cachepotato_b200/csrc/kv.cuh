@@ -20,7 +20,8 @@ struct KvView {
 struct KvRows {
     int n, T;
     const int *q_start, *pos0, *pages;
-    int table_stride, max_pages;
+    int table_stride;
+    int cap;                         // positions a sequence may have: the table's, and what 32 bits count
 };
 
 // Tensor maps of the two pools: axes (element, place, head, page), a box of 128 bytes by `box`
@@ -84,7 +85,7 @@ struct KvSeq {
     int r0, len, p0;
     bool bad;
 };
-__device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int P, int i) {
+__device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int i) {
     KvSeq s;
     const int a = b.q_start[i], e = b.q_start[i + 1];
     s.r0 = a;
@@ -92,9 +93,8 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int P, int i) {
     s.len = 0;
     s.bad = a < 0 || e < a || e > b.T || (e > a && s.p0 < 0);    // (no rows: pos0 may be anything)
     if (a >= 0 && s.p0 >= 0 && min(e, b.T) > a) {
-        const long cap = min((long)b.max_pages * P, 0x7fff0000l);   // positions and tile ends stay in 32 bits
         const int n = min(e, b.T) - a;
-        s.len = (int)min((long)n, max(0l, cap - s.p0));
+        s.len = min(n, max(0, b.cap - s.p0));
         s.bad = s.bad || s.len < n;
     }
     return s;

@@ -148,7 +148,7 @@ struct KdRows {
 template <int ROWS>
 __device__ __forceinline__ KdSeq kd_seq(const AttendArgs &a, int G, int i) {
     KdSeq q;
-    q.s = kv_seq(a.b, a.c.P, i);
+    q.s = kv_seq(a.b, i);
     q.rt = (int)(((long)q.s.len * G + ROWS - 1) / ROWS);
     long tiles = 0;
     for (int r = 0; r < q.rt; ++r) tiles += KD_FIXED + KdRows<ROWS>(a, G, q.s, r).nt;
@@ -171,7 +171,7 @@ struct KdCursor {
             rt = 0;
             do {
                 if (++seq >= a.b.n) return;
-                s = kv_seq(a.b, a.c.P, seq);
+                s = kv_seq(a.b, seq);
             } while (s.len == 0);
             n_rt = (int)(((long)s.len * G + ROWS - 1) / ROWS);
         }

@@ -27,7 +27,7 @@ __device__ __forceinline__ int kt_tiles(const AttendArgs &a, int Q, const KvSeq 
 template <int TILE, int FIXED>
 __device__ __forceinline__ KtSeq kt_seq(const AttendArgs &a, int Q, int i) {
     KtSeq q;
-    q.s = kv_seq(a.b, a.c.P, i);
+    q.s = kv_seq(a.b, i);
     q.pairs = (q.s.len + Q - 1) / Q;
     q.head_units = 0;
     // a handful of instructions a pair; a closed form took longer than summing thousands of pairs
@@ -62,7 +62,7 @@ struct KtCursor {
             kh = 0;
             do {
                 if (++seq >= a.b.n) return;
-                s = kv_seq(a.b, a.c.P, seq);
+                s = kv_seq(a.b, seq);
             } while (s.len == 0);
             pairs = (s.len + Q - 1) / Q;
         }

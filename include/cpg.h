@@ -338,7 +338,8 @@ typedef struct {
     int n_seqs, rows;                    /* rows of q, k, v and out */
     const int *q_start;                  /* (n_seqs + 1), ascending */
     const int *pos0;                     /* (n_seqs) position of the first new row (no rows: anything) */
-    const int *pages;                    /* (n_seqs, max_pages) page ids, rows table_stride apart */
+    const int *pages;                    /* (n_seqs, max_pages) page ids, rows table_stride apart;
+                                            positions end at 2^31 - 2^16 and at 2^36 / n_kv */
     int table_stride, max_pages;
     int max_new;                         /* most new rows of a sequence; 0: not known, taken as `rows`.
                                             Chooses the kernel only: any value gives right results, but

@@ -395,6 +395,27 @@ def test_attend_counts_every_position_once(rt, ct, hd, new):
         close(got, want, off * want + tiny(TYPES[rt]), f"window {window}")
 
 
+@pytest.mark.parametrize("rt,ct", COMBOS)
+@pytest.mark.parametrize("new", [1, 80])
+def test_one_page_many_times(rt, ct, new):
+    """Many cached heads over a long table that names the same page again and again: what a row sees is that
+    page's positions over and over, so the result is the page's own."""
+    from cachepotato_b200.kv import KVBatch, KVCache
+    page, KV, hd, times = 64, 128 if new == 1 else 16, 64, 1500
+    one = R.Batch([(1, page - 1)], page, 3, spare=0)
+    kp, vp = R.pools(one, KV, hd, TYPES[ct], 4)
+    q = rows((1, 2 * KV, hd), TYPES[rt], 5).repeat(new, 1, 1)
+    want, size = R.attend(one, q[:1], kp, vp, hd ** -0.5, 0)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    arrays = (torch.arange(new + 1, **i32), torch.full((new,), page * times - 1, **i32), torch.zeros((new, times), **i32))
+    cache = KVCache(kp, vp, rope_dim=0)
+    tol = attend_tol(R.Batch([(1, page * times)], page, 3), want, size, vp, TYPES[rt])
+    for hint in (1, 80):                                          # single rows on both kinds of kernel
+        got = cache.attend(KVBatch(*arrays, rows=new, max_new=hint), q)
+        cache.check()
+        close(got, want.repeat(new, 1, 1), tol.repeat(new, 1, 1), f"hint {hint}")
+
+
 def test_attend_scale_and_in_place():
     from cachepotato_b200.kv import KVCache
     for rt, ct in COMBOS:
