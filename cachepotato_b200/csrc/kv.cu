@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(128, AP_BLOCKS) k_kv_append(const __grid_const
     }
     // every sequence is looked at once, whether a row leads to it or not; the last warps first, which
     // have no row to find where there are few
-    for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x + 1) * blockDim.x - 1 - tid; i < a.b.n; i += (size_t)gridDim.x * gridDim.y * blockDim.x)
+    const size_t all = (size_t)gridDim.x * gridDim.y * blockDim.x;
+    for (size_t i = ((size_t)blockIdx.y * gridDim.x + blockIdx.x + 1) * blockDim.x - 1 - tid; i < a.b.n; i += all)
         if (kv_seq(a.b, (int)i).bad) atomicOr(a.c.status, KV_BAD_POS);
     float gq[2 * E];
     auto gains = [&](const float *g, float *to) {

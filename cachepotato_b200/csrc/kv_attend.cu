@@ -31,9 +31,9 @@
 //           for the tiles in flight, 15 us where a block ends an item in the middle of its range.
 //   measured  (on the device, calls in a captured graph) 128 bf16 rows over 1000-8000 positions (1.14 GB):
 //           187 us, 0.93 of the copy bandwidth; 64 f32 rows over f16, 128-4096 positions (294 MB): 56 us,
-//           0.80 (59 from call to call), over bf16 60 us, over f32 (586 MB) 113 us, 0.80; one bf16 row over 128K positions
-//           (268 MB): 59 us, 0.70 (4.5 us until the first tile, 41 of tiles at the copy bandwidth, the
-//           rest the joins of 74 parts); one f32 row over 512 positions: 11 us.
+//           0.80 (59 from call to call), over bf16 60 us, over f32 (586 MB) 113 us, 0.80; one bf16
+//           row over 128K positions (268 MB): 59 us, 0.70 (4.5 us until the first tile, 41 of tiles at the
+//           copy bandwidth, the rest the joins of 74 parts); one f32 row over 512 positions: 11 us.
 //   types   16-bit rows: one product per step, P rounded to the cache's type (its rounding is as
 //           large as the result's own). f32 rows keep about 22 bits: over an f16 cache q (scaled by
 //           a power of two per row, as far up as f16 goes: the small elements of a row with a large one

@@ -359,8 +359,8 @@ int cpg_kv_append(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads
  * window > 0 only to j > p - window; n_heads a multiple of n_kv, consecutive heads sharing a cached
  * one; weights softmax(scale q·k). Positions that no row of a sequence sees, behind its last row or in
  * front of its first row's window, take no part, whatever the pages hold there. A position that only
- * some rows of a sequence see takes part in the others' sums with weight zero, so its value must be finite; f32 rows are split into 16-bit terms, so
- * they and what they see must be finite too. out may be q.
+ * some rows of a sequence see takes part in the others' sums with weight zero, so its value must be
+ * finite; f32 rows are split into 16-bit terms, so they and what they see must be finite too. out may be q.
  * f32 rows: products to about 22 bits, f32 sums. 16-bit rows: the weights are rounded to the
  * cache's type before the sum over values, which accumulates in f32 (f16: lifted by a power of two
  * first, so that a long cache's small weights do not vanish).
@@ -372,7 +372,8 @@ int cpg_kv_attend(const cpg_kv *kv, const cpg_kv_batch *b, int type, int n_heads
 /* Synchronise `stream` and report, once, what the calls since the last check met: CPG_EINVAL if a
  * page id lay outside the pool, or rows or positions outside the batch or its table, or a sequence
  * ended before it began (such keys and values were not written, and what the rows that see them hold
- * is not specified; no memory outside the pools and the rows was touched), CPG_ETIMEOUT if a bounded device wait gave up. */
+ * is not specified; no memory outside the pools and the rows was touched), CPG_ETIMEOUT if a bounded
+ * device wait gave up. */
 int cpg_kv_check(const cpg_kv *kv, void *stream);
 
 /* ------------------------------------------- many sequences over a pool of pages
@@ -381,7 +382,8 @@ int cpg_kv_check(const cpg_kv *kv, void *stream);
  * holds pages for the positions it has, so n_slots times max_ctx may be far more than the pool; a step
  * that needs more pages than are free is refused with CPG_ENOMEM and changes nothing. With an f32
  * cache the ids per sequence are those of cpg_qwen3_generate; a 16-bit one rounds keys and values.
- * After an error no position has moved, so the call can be repeated. Runs on the model's stream and scratch: not at the same time as its own sequence or a batch. */
+ * After an error no position has moved, so the call can be repeated.
+ * Runs on the model's stream and scratch: not at the same time as its own sequence or a batch. */
 typedef struct cpg_qwen3_paged cpg_qwen3_paged;
 int cpg_qwen3_paged_create(cpg_qwen3 *m, int n_slots, int max_ctx, int page_size, int n_pages, int type,
                            cpg_qwen3_paged **out);
